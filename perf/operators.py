@@ -15,7 +15,8 @@ power of two as scale, the smallest that keeps the block's largest value within 
 stored as one of them by a given random number: m so that its expectation is m, the root so that the expectation of
 its square is v; a v that is not zero is not stored as zero. The random number of element i of tensor k in the step
 with seed s is ``word = mix(i + mix(s + k * 0x9E3779B1))``, its low half for m, its high half for the root, and for a
-parameter in bf16 the low half of ``mix(word ^ 0x5BF03635)``, added below the 16 bits that stay.
+parameter in bf16 the low half of ``mix(word ^ 0x5BF03635)``, added below the 16 bits that stay. A half h chooses
+the upper code where ``(h + 0.5) / 65536`` is less than the share of the way.
 """
 
 import itertools
@@ -359,7 +360,7 @@ def _write_codes(x, chance, codes, scales, squares):
     share, whole = size - below, step
     if squares:
         share, whole = share * (size + below), step * (below + below + step)
-    size = below + torch.where(chance.float() * whole < share * 65536, step, 0)
+    size = below + torch.where((chance.float() + 0.5) * whole < share * 65536, step, 0)
     codes.copy_(torch.copysign(size, x))
     scales.view(torch.uint8).copy_(k)
 
@@ -434,7 +435,7 @@ def exact(case, seed):
             out["v"][here] = v
         else:
             word = mixed(torch.arange(p.numel(), device="cuda") + mixed(t + k * 0x9E3779B1 & 0xFFFFFFFF) & 0xFFFFFFFF)
-            m, out["root"][here] = stored(m, (word % 65536) / 65536, 1), stored(torch.sqrt(v), (word // 65536) / 65536, 2)
+            m, out["root"][here] = stored(m, (word % 65536 + 0.5) / 65536, 1), stored(torch.sqrt(v), (word // 65536 + 0.5) / 65536, 2)
             if case["param"] == "bf16":
                 ulp = torch.exp2(torch.floor(torch.log2(p.abs().clamp(min=2.0**-126))) - 7)
                 p = torch.sign(p) * ulp * torch.floor(p.abs() / ulp + (mixed(word ^ 0x5BF03635) % 65536) / 65536)
