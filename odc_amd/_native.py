@@ -33,6 +33,12 @@ TORCH_BINDING_SOURCE = CSRC_DIR / "odc_torch.cpp"
 CEILING_LIB_PATH = CSRC_DIR / "libodc_ceiling.so"
 CEILING_SOURCES = [CSRC_DIR / "ceiling_kernels.hip"]
 
+# the operators of odc_amd.ops (include/odc_ops.h): a library and an extension of their own, built the same way
+OPS_LIB_PATH = CSRC_DIR / "libodc_ops.so"
+OPS_SOURCES = [CSRC_DIR / "odc_ops_host.cpp", CSRC_DIR / "odc_norm_kernels.hip", CSRC_DIR / "odc_adamw_kernels.hip"]
+OPS_BINDING_PATH = CSRC_DIR / "odc_ops_torch.so"
+OPS_BINDING_SOURCE = CSRC_DIR / "odc_ops_torch.cpp"
+
 # every symbol include/odc_hip.h declares
 EXPORTED_SYMBOLS = (
     "odc_arena_create",
@@ -56,7 +62,21 @@ EXPORTED_SYMBOLS = (
     "odc_get_option",
 )
 
+# every symbol include/odc_ops.h declares
+OPS_EXPORTED_SYMBOLS = (
+    "odc_layer_norm",
+    "odc_layer_norm_backward",
+    "odc_layer_norm_backward_workspace",
+    "odc_squared_norm",
+    "odc_squared_norm_workspace",
+    "odc_adamw",
+    "odc_dequantize_blocks",
+    "odc_ops_last_error",
+    "odc_ops_abi_version",
+)
+
 ABI_VERSION = 3
+OPS_ABI_VERSION = 1
 MAX_ITEMS_PER_LAUNCH = 112
 
 ODC_OK = 0
@@ -203,11 +223,16 @@ def build_ceiling_library(verbose: bool = False) -> Path:
     return _compile(CEILING_LIB_PATH, lambda output: hipcc_command(output, CEILING_SOURCES), verbose)
 
 
-def _torch_binding_target() -> str:
-    """What odc_torch.so is built for: it reads at::Tensor and CPython objects by their layout."""
+def build_ops_library(verbose: bool = False) -> Path:
+    """Compile libodc_ops.so in-tree for gfx950 (works without a GPU)."""
+    return _compile(OPS_LIB_PATH, lambda output: hipcc_command(output, OPS_SOURCES), verbose)
+
+
+def _torch_binding_target(abi_version: int = None) -> str:
+    """What odc_torch.so (odc_ops_torch.so) is built for: it reads at::Tensor and CPython objects by their layout."""
     import torch
 
-    return f"ABI {ABI_VERSION}, torch {torch.__version__}, CPython {sys.version_info.major}.{sys.version_info.minor}"
+    return f"ABI {abi_version or ABI_VERSION}, torch {torch.__version__}, CPython {sys.version_info.major}.{sys.version_info.minor}"
 
 
 def torch_binding_command(output: Path = TORCH_BINDING_PATH) -> list[str]:
@@ -229,20 +254,33 @@ def build_torch_binding(verbose: bool = False) -> Path:
     return _compile(TORCH_BINDING_PATH, torch_binding_command, verbose)
 
 
+def ops_binding_command(output: Path = OPS_BINDING_PATH) -> list[str]:
+    command = torch_binding_command(output)
+    command[command.index(str(TORCH_BINDING_SOURCE))] = str(OPS_BINDING_SOURCE)
+    # it asks torch for the current stream, which is torch's HIP library's to know
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    return [*command, "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-I{rocm / 'include'}", "-lc10_hip"]
+
+
+def build_ops_binding(verbose: bool = False) -> Path:
+    """Compile odc_ops_torch.so in-tree."""
+    return _compile(OPS_BINDING_PATH, ops_binding_command, verbose)
+
+
 _REBUILD = "run `python -c 'import __graft_entry__ as g; g.build()'`"
 _torch_binding = None
 
 
-def _load_torch_binding_file(path: Path):
+def _load_torch_binding_file(path: Path, name: str = "odc_torch", abi_version: int = None):
     """The extension module at ``path``; ImportError when it was built for something else."""
-    loader = importlib.machinery.ExtensionFileLoader("odc_torch", str(path))
-    spec = importlib.util.spec_from_file_location("odc_torch", path, loader=loader)
+    loader = importlib.machinery.ExtensionFileLoader(name, str(path))
+    spec = importlib.util.spec_from_file_location(name, path, loader=loader)
     try:
         module = importlib.util.module_from_spec(spec)
         loader.exec_module(module)
     except ImportError as e:  # a symbol of another torch, or not a library at all
         raise ImportError(f"{path} cannot be loaded ({e}): {_REBUILD}") from None
-    built_for, wanted = getattr(module, "built_for", "something older"), _torch_binding_target()
+    built_for, wanted = getattr(module, "built_for", "something older"), _torch_binding_target(abi_version)
     if built_for != wanted:
         raise ImportError(f"{path} is stale: built for {built_for}, this is {wanted}: {_REBUILD}")
     return module
@@ -268,6 +306,49 @@ def load_torch_binding():
             module.bind(*entry_points)
             _torch_binding = module
     return _torch_binding
+
+
+_ops_lib = None
+_ops_binding = None
+
+
+def _open_ops_library(path: Path) -> ctypes.CDLL:
+    import torch  # noqa: F401  its HIP runtime comes first, as in load()
+
+    lib = ctypes.CDLL(str(path))
+    for name in OPS_EXPORTED_SYMBOLS:
+        if not hasattr(lib, name):
+            raise ImportError(f"{path} is stale (no {name}): rebuild it")
+    lib.odc_ops_last_error.restype = ctypes.c_char_p
+    for name in ("odc_layer_norm_backward_workspace", "odc_squared_norm_workspace"):
+        getattr(lib, name).restype = ctypes.c_uint64
+    got = lib.odc_ops_abi_version()
+    if got != OPS_ABI_VERSION:
+        raise ImportError(f"{path} has ABI version {got}, expected {OPS_ABI_VERSION}: rebuild it")
+    return lib
+
+
+def load_ops():
+    """The extension module of odc_ops_torch.cpp, bound to libodc_ops.so; both are built on first use when missing.
+    There is no Python or CPU path behind it."""
+    global _ops_lib, _ops_binding
+    with _lib_lock:
+        if _ops_binding is None:
+            for path, build in ((OPS_LIB_PATH, build_ops_library), (OPS_BINDING_PATH, build_ops_binding)):
+                if not path.exists():
+                    try:
+                        build()
+                    except (OSError, RuntimeError) as e:
+                        raise ImportError(f"{path} is missing and could not be built ({e}): {_REBUILD}") from None
+            _ops_lib = _open_ops_library(OPS_LIB_PATH)
+            module = _load_torch_binding_file(OPS_BINDING_PATH, "odc_ops_torch", OPS_ABI_VERSION)
+            entry_points = []
+            for name in OPS_EXPORTED_SYMBOLS:
+                if name != "odc_ops_abi_version":
+                    entry_points += [name, ctypes.cast(getattr(_ops_lib, name), ctypes.c_void_p).value]
+            module.bind(*entry_points)
+            _ops_binding = module
+    return _ops_binding
 
 
 def load_ceiling() -> ctypes.CDLL:

@@ -1,0 +1,82 @@
+// odc_ops_launch.h — what the host side of libodc_ops.so (odc_ops_host.cpp, plain C++: the C ABI, the checks
+// and the launch plans) hands to its device side (odc_norm_kernels.hip, odc_adamw_kernels.hip). The
+// descriptors travel BY VALUE in the kernel-argument segment. A second implementation of namespace
+// odc_ops_device without a device (tests/cpu/no_ops_device.cpp) lets the host side run under
+// AddressSanitizer and UBSan on the CPU.
+#ifndef ODC_OPS_LAUNCH_H_
+#define ODC_OPS_LAUNCH_H_
+
+#include <stdint.h>
+
+#include "odc_ops.h"
+
+namespace odc_ops_launch {
+
+inline bool is_float_type(int32_t dtype) { return dtype == ODC_OPS_BF16 || dtype == ODC_OPS_F16 || dtype == ODC_OPS_F32; }
+inline uint32_t bytes_of(int32_t dtype) { return dtype == ODC_OPS_F32 ? 4 : 2; }
+
+// ---- layer norm -----------------------------------------------------------------------------------
+constexpr uint32_t kNormThreads = 256;
+// The gradients of weight and bias are sums over the rows. `groups` workgroups add up rows of their own, each
+// into its row of the workspace ([groups][2][width] floats), and a second launch adds the groups.
+constexpr uint32_t kColumnTile = 64;  // columns of one workgroup of the column sums
+constexpr uint32_t kMostGroups = 256;
+
+struct NormForwardPlan {
+  uint32_t blocks;
+};
+
+struct NormBackwardPlan {
+  uint32_t row_blocks;  // workgroups of the pass over rows
+  uint32_t groups;
+  uint64_t rows_per_group;
+};
+
+// ---- lists of tensors -----------------------------------------------------------------------------
+// A dispatch counts its work-items in 32 bits: the most workgroups of 256.
+constexpr uint32_t kMostTiles = 0xffffffffu / 256;
+// A launch has a table of its tensors and the number of the first tile of each.
+constexpr uint32_t kNormItems = 160;
+constexpr uint32_t kNormTile = 8192;  // elements of a tile of the squared norm
+constexpr uint32_t kMostPartials = 2048;
+struct SquaredNormLaunch {
+  uint32_t n_items, n_tiles;
+  uint32_t first_tile[kNormItems + 1];
+  odc_span_item items[kNormItems];
+};
+static_assert(sizeof(SquaredNormLaunch) <= 3800, "kernel arguments are limited to 4 KiB");
+
+constexpr uint32_t kBlock = 32;  // elements of a state in 8 bits that share a scale
+constexpr uint32_t kAdamwItems = 48;
+constexpr uint32_t kAdamwTile = 1024;  // elements
+constexpr uint32_t kAdamwThreads = 256;
+struct AdamwLaunch {
+  float beta1, beta2, one_minus_beta1, one_minus_beta2;
+  float decay;          // 1 - lr * weight_decay
+  float step_size;      // lr / (1 - beta1^t)
+  float root_scale;     // 1 / sqrt(1 - beta2^t)
+  float eps, grad_scale, max_norm;
+  const float* squared_norm;
+  uint32_t seed, first_item, stochastic;
+  uint32_t n_items, n_tiles;
+  uint32_t first_tile[kAdamwItems + 1];
+  odc_adamw_item items[kAdamwItems];
+};
+static_assert(sizeof(AdamwLaunch) <= 3800, "kernel arguments are limited to 4 KiB");
+
+}  // namespace odc_ops_launch
+
+namespace odc_ops_device {
+
+// Each returns 0 or a hipError_t.
+int launch_norm_forward(const odc_norm_forward& call, const odc_ops_launch::NormForwardPlan& plan, void* stream);
+int launch_norm_backward(const odc_norm_backward& call, const odc_ops_launch::NormBackwardPlan& plan, void* stream);
+int launch_squared_norm(int32_t dtype, const odc_ops_launch::SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream);
+int launch_squared_norm_total(const double* partials, uint32_t n, float* result, void* stream);
+int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, const odc_ops_launch::AdamwLaunch& launch, void* stream);
+int launch_dequantize(const void* codes, const void* scales, void* values, uint64_t elems, int32_t dtype, void* stream);
+const char* error_string(int code);
+
+}  // namespace odc_ops_device
+
+#endif  // ODC_OPS_LAUNCH_H_
