@@ -7,11 +7,280 @@ namespace {
 
 using namespace odc_ops_launch;
 
+// ------------------------------------------------------------------------------------------------
+// rows in registers
+// ------------------------------------------------------------------------------------------------
+// kElems neighbouring elements of a row from element i on; what lies behind the row's end is zero, and not read.
+template <int kElems, class T>
+struct Piece {
+  static constexpr int kVectors = kElems / Vector<T>::kElems;
+  typename Vector<T>::type v[kVectors];
+
+  __device__ __forceinline__ void load(const T* row, uint32_t i, uint32_t width) {
+    if (i + kElems <= width) {
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k) v[k] = *reinterpret_cast<const typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) set(e, i + e < width ? row[i + e] : (T)0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(T* row, uint32_t i, uint32_t width) const {
+    if (i + kElems <= width) {
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k) *reinterpret_cast<typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems) = v[k];
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e)
+        if (i + e < width) row[i + e] = v[e / Vector<T>::kElems][e % Vector<T>::kElems];
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return to_float(v[e / Vector<T>::kElems][e % Vector<T>::kElems]); }
+  __device__ __forceinline__ void set(int e, T x) { v[e / Vector<T>::kElems][e % Vector<T>::kElems] = x; }
+  // What was computed from it so far is forgotten: the compiler would keep the converted values over a barrier, in
+  // twice the registers, where converting them again costs an instruction each.
+  __device__ __forceinline__ void forget() {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) asm("" : "+v"(reinterpret_cast<u32x4&>(v[k])));
+  }
+};
+
+// The sums of kValues values over the lanes of a row. More than a wavefront's meet in LDS: `scratch` has kValues floats
+// for every wavefront, and the caller alternates between two of them, so that one barrier is enough.
+template <int kLanes, int kValues>
+__device__ __forceinline__ void row_sums(float (&x)[kValues], float* scratch) {
+#pragma unroll
+  for (int v = 0; v < kValues; ++v) x[v] = sum_lanes<(kLanes < 64 ? kLanes : 64)>(x[v]);
+  if constexpr (kLanes > 64) {
+    const uint32_t wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) {
+#pragma unroll
+      for (int v = 0; v < kValues; ++v) scratch[wave * kValues + v] = x[v];
+    }
+    __syncthreads();
+    const float* mine = scratch + wave / (kLanes / 64) * (kLanes / 64) * kValues;
+#pragma unroll
+    for (int v = 0; v < kValues; ++v) {
+      x[v] = mine[v];
+#pragma unroll
+      for (int w = 1; w < kLanes / 64; ++w) x[v] += mine[w * kValues + v];
+    }
+  }
+}
+
+template <class T, class W, int kLanes, int kVectors, bool kAdd>
+__global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads) void norm_forward_kernel(odc_norm_forward c) {
+  constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
+  constexpr int kElems = Vector<T>::kElems;
+  __shared__ float scratch[2][kThreads / 64];
+  const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes;
+  const float per_element = 1.0f / (float)width;
+  Piece<kElems, W> weight[kVectors], bias[kVectors];
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    const uint32_t i = (k * kLanes + lane) * kElems;
+    if (c.weight) {
+      weight[k].load(static_cast<const W*>(c.weight), i, width);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) weight[k].set(e, (W)1.0f);
+    }
+    if (c.bias) {
+      bias[k].load(static_cast<const W*>(c.bias), i, width);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) bias[k].set(e, (W)0.0f);
+    }
+  }
+  constexpr uint32_t kRows = kThreads / kLanes;  // at once
+  uint64_t row = (uint64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
+  Piece<kElems, T> x[kVectors], r[kVectors];
+  const auto load = [&](Piece<kElems, T>(&piece)[kVectors], const void* rows, uint64_t stride) {
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows ? width : 0);
+  };
+  const auto load_row = [&](Piece<kElems, T>(&piece)[kVectors]) {
+    load(piece, c.input, c.input_stride);
+    if constexpr (kAdd) load(r, c.residual, c.residual_stride);
+  };
+  constexpr bool kAhead = kVectors <= 2;  // with more the registers are full
+  if constexpr (kAhead) load_row(x);
+  while (row < c.rows) {
+    if constexpr (!kAhead) load_row(x);
+    if constexpr (kAdd) {
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k) {
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) x[k].set(e, from_float<T>(x[k][e] + r[k][e]));
+        x[k].store(static_cast<T*>(c.total) + row * c.width, (k * kLanes + lane) * kElems, width);
+      }
+    }
+    float sum[1] = {};
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) sum[0] += x[k][e];
+    const uint64_t here = row;
+    Piece<kElems, T> next[kVectors];
+    row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
+    if constexpr (kAhead) load_row(next);
+    row_sums<kLanes>(sum, scratch[0]);
+    const float mean = sum[0] / (float)width;  // (times 1 / width a row of one value would not have it for a mean)
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) x[k].forget();
+    float squares[1] = {};
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const float d = (k * kLanes + lane) * kElems + e < width ? x[k][e] - mean : 0.0f;
+        squares[0] += d * d;
+      }
+    row_sums<kLanes>(squares, scratch[1]);
+    const float rstd = 1.0f / sqrtf(squares[0] * per_element + c.eps);
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      x[k].forget();
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) x[k].set(e, from_float<T>((x[k][e] - mean) * rstd * weight[k][e] + bias[k][e]));
+      x[k].store(static_cast<T*>(c.output) + here * c.width, (k * kLanes + lane) * kElems, width);
+      if constexpr (kAhead) x[k] = next[k];
+    }
+    if (lane == 0) {
+      if (c.mean) c.mean[here] = mean;
+      if (c.rstd) c.rstd[here] = rstd;
+    }
+  }
+}
+
+// A workgroup passes over rows blockIdx.x, + gridDim.x, ... (kThreads / kLanes of them at once), writes their
+// grad_input and keeps the sums for weight and bias of its lanes' columns in registers; at the end the rows that it had
+// at once are added in LDS, upper half onto lower half, and go to its row of the workspace.
+template <class T, class W, int kLanes, int kVectors>
+__global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_norm_backward c) {
+  constexpr int kThreads = kBackwardThreads, kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
+  constexpr int kSums = 2 * kVectors * kElems;  // of a thread
+  __shared__ float scratch[2][2 * kThreads / 64];
+  __shared__ float upper[kRows > 1 ? kThreads / 2 * kSums : 1];
+  const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const float per_element = 1.0f / (float)width;
+  const bool sums = c.grad_weight || c.grad_bias;
+  Piece<kElems, W> weight[kVectors];
+  float dw[kVectors][kElems] = {}, db[kVectors][kElems] = {};
+  const auto load_weight = [&]() {
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      if (c.weight) {
+        weight[k].load(static_cast<const W*>(c.weight), (k * kLanes + lane) * kElems, width);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) weight[k].set(e, (W)1.0f);
+      }
+    }
+  };
+  // With one vector to a lane there are registers for the weights and for a row ahead; with two the weights are read
+  // again from the caches.
+  constexpr bool kAhead = kVectors == 1;
+  if constexpr (kAhead) load_weight();
+  int parity = 0;
+  uint64_t row = (uint64_t)blockIdx.x * kRows + slot;
+  Piece<kElems, T> x[kVectors], dy[kVectors], dt[kVectors];
+  float mean, rstd;
+  const auto load = [&](Piece<kElems, T>(&piece)[kVectors], const void* rows, uint64_t stride) {
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+      piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows && rows ? width : 0);
+  };
+  const auto load_row = [&]() {
+    load(dy, c.grad_output, c.grad_output_stride);
+    load(x, c.normalised, c.normalised_stride);
+    mean = row < c.rows ? c.mean[row] : 0;
+    rstd = row < c.rows ? c.rstd[row] : 0;
+  };
+  if constexpr (kAhead) load_row();
+  // every thread makes the same number of rounds: there are barriers in them
+  for (uint64_t first = (uint64_t)blockIdx.x * kRows; first < c.rows; first += (uint64_t)gridDim.x * kRows, parity ^= 1) {
+    if constexpr (!kAhead) {
+      load_row();
+      load_weight();
+    }
+    if (c.grad_input) load(dt, c.grad_total, c.grad_total_stride);
+    float row_sum[2] = {};
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const float z = (x[k][e] - mean) * rstd, g = dy[k][e];  // behind the row's end g is zero and z of no account
+        const float h = g * weight[k][e];
+        row_sum[0] += h;
+        row_sum[1] += h * z;
+        dw[k][e] += g * z;
+        db[k][e] += g;
+      }
+    const uint64_t here = row;
+    const float mean_here = mean, rstd_here = rstd;
+    Piece<kElems, T> x_here[kVectors], dy_here[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) x_here[k] = x[k], dy_here[k] = dy[k];
+    row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
+    if constexpr (kAhead) load_row();
+    if (c.grad_input) {
+      row_sums<kLanes>(row_sum, scratch[parity]);
+      const float sum = row_sum[0] * per_element, dot = row_sum[1] * per_element;
+      if (here < c.rows) {
+        if constexpr (!kAhead) load_weight();
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+          x_here[k].forget();
+          dy_here[k].forget();
+#pragma unroll
+          for (int e = 0; e < kElems; ++e) {
+            const float z = (x_here[k][e] - mean_here) * rstd_here, h = dy_here[k][e] * weight[k][e];
+            x_here[k].set(e, from_float<T>(rstd_here * (h - sum - z * dot) + dt[k][e]));
+          }
+          x_here[k].store(static_cast<T*>(c.grad_input) + here * c.width, (k * kLanes + lane) * kElems, width);
+        }
+      }
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int half = kThreads / 2; half >= kLanes; half /= 2) {
+    if (threadIdx.x >= (uint32_t)half && threadIdx.x < 2u * half) {
+#pragma unroll
+      for (int s = 0; s < kSums; ++s) upper[s * half + threadIdx.x - half] = s % 2 ? db[s / 2 / kElems][s / 2 % kElems] : dw[s / 2 / kElems][s / 2 % kElems];
+    }
+    __syncthreads();
+    if (threadIdx.x < (uint32_t)half) {
+#pragma unroll
+      for (int s = 0; s < kSums; ++s) (s % 2 ? db[s / 2 / kElems][s / 2 % kElems] : dw[s / 2 / kElems][s / 2 % kElems]) += upper[s * half + threadIdx.x];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < (uint32_t)kLanes) {
+    float* out = static_cast<float*>(c.workspace) + (uint64_t)blockIdx.x * 2 * width;
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const uint32_t i = (k * kLanes + lane) * kElems + e;
+        if (i < width) {
+          out[i] = dw[k][e];
+          out[width + i] = db[k][e];
+        }
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// wide rows
+// ------------------------------------------------------------------------------------------------
 // One workgroup per row, three passes over it (the second and third find it in the caches): the mean, the
 // variance about that mean, the output.
 template <class T, class W>
-__global__ __launch_bounds__(kNormThreads) void norm_forward_kernel(odc_norm_forward c) {
-  __shared__ float scratch[kNormThreads / 64];
+__global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_norm_forward c) {
+  __shared__ float scratch[kWideThreads / 64];
   const W* weight = static_cast<const W*>(c.weight);
   const W* bias = static_cast<const W*>(c.bias);
   for (uint64_t row = blockIdx.x; row < c.rows; row += gridDim.x) {
@@ -20,7 +289,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_forward_kernel(odc_norm_for
     T* y = static_cast<T*>(c.output) + row * c.width;
     T* total = r ? static_cast<T*>(c.total) + row * c.width : nullptr;
     float sum = 0;
-    for (uint64_t i = threadIdx.x; i < c.width; i += kNormThreads) {
+    for (uint64_t i = threadIdx.x; i < c.width; i += kWideThreads) {
       float v = to_float(x[i]);
       if (r) {
         const T t = from_float<T>(v + to_float(r[i]));
@@ -30,14 +299,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_forward_kernel(odc_norm_for
       sum += v;
     }
     const T* z = r ? total : x;  // a thread reads what it wrote itself
-    const float mean = block_sum<kNormThreads>(sum, scratch) / (float)c.width;
+    const float mean = block_sum<kWideThreads>(sum, scratch) / (float)c.width;
     float squares = 0;
-    for (uint64_t i = threadIdx.x; i < c.width; i += kNormThreads) {
+    for (uint64_t i = threadIdx.x; i < c.width; i += kWideThreads) {
       const float d = to_float(z[i]) - mean;
       squares += d * d;
     }
-    const float rstd = 1.0f / sqrtf(block_sum<kNormThreads>(squares, scratch) / (float)c.width + c.eps);
-    for (uint64_t i = threadIdx.x; i < c.width; i += kNormThreads) {
+    const float rstd = 1.0f / sqrtf(block_sum<kWideThreads>(squares, scratch) / (float)c.width + c.eps);
+    for (uint64_t i = threadIdx.x; i < c.width; i += kWideThreads) {
       float v = (to_float(z[i]) - mean) * rstd;
       if (weight) v *= to_float(weight[i]);
       if (bias) v += to_float(bias[i]);
@@ -51,8 +320,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_forward_kernel(odc_norm_for
 }
 
 template <class T, class W>
-__global__ __launch_bounds__(kNormThreads) void norm_backward_rows_kernel(odc_norm_backward c) {
-  __shared__ float scratch[kNormThreads / 64];
+__global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_norm_backward c) {
+  __shared__ float scratch[kWideThreads / 64];
   const W* weight = static_cast<const W*>(c.weight);
   for (uint64_t row = blockIdx.x; row < c.rows; row += gridDim.x) {
     const T* dy = static_cast<const T*>(c.grad_output) + row * c.grad_output_stride;
@@ -61,14 +330,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_rows_kernel(odc_no
     T* dx = static_cast<T*>(c.grad_input) + row * c.width;
     const float mean = c.mean[row], rstd = c.rstd[row];
     float sum = 0, dot = 0;
-    for (uint64_t i = threadIdx.x; i < c.width; i += kNormThreads) {
+    for (uint64_t i = threadIdx.x; i < c.width; i += kWideThreads) {
       const float h = to_float(dy[i]) * (weight ? to_float(weight[i]) : 1.0f);
       sum += h;
       dot += h * ((to_float(x[i]) - mean) * rstd);
     }
-    sum = block_sum<kNormThreads>(sum, scratch) / (float)c.width;
-    dot = block_sum<kNormThreads>(dot, scratch) / (float)c.width;
-    for (uint64_t i = threadIdx.x; i < c.width; i += kNormThreads) {
+    sum = block_sum<kWideThreads>(sum, scratch) / (float)c.width;
+    dot = block_sum<kWideThreads>(dot, scratch) / (float)c.width;
+    for (uint64_t i = threadIdx.x; i < c.width; i += kWideThreads) {
       const float h = to_float(dy[i]) * (weight ? to_float(weight[i]) : 1.0f);
       const float z = (to_float(x[i]) - mean) * rstd;
       float d = rstd * (h - sum - z * dot);
@@ -80,8 +349,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_rows_kernel(odc_no
 
 // Workgroup (tile of columns, group of rows): the sums over the group's rows. Wavefront w takes every fourth row.
 template <class T>
-__global__ __launch_bounds__(kNormThreads) void norm_backward_columns_kernel(odc_norm_backward c, uint64_t rows_per_group) {
-  constexpr int kWaves = kNormThreads / 64;
+__global__ __launch_bounds__(kWideThreads) void norm_backward_columns_kernel(odc_norm_backward c, uint64_t rows_per_group) {
+  constexpr int kWaves = kWideThreads / 64;
   __shared__ float scratch[2][kWaves][64];
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const uint64_t column = (uint64_t)blockIdx.x * kColumnTile + lane;
@@ -106,16 +375,43 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_columns_kernel(odc
   }
 }
 
+// The sums over the groups: 64 columns of [2][width] and 16 groups at once, four columns to a thread.
 template <class W>
-__global__ __launch_bounds__(kNormThreads) void norm_backward_groups_kernel(odc_norm_backward c, uint32_t groups) {
-  const uint64_t at = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x;  // of [2][width]
-  if (at >= 2 * c.width) return;
-  float sum = 0;
-  for (uint32_t g = 0; g < groups; ++g) sum += static_cast<const float*>(c.workspace)[g * 2 * c.width + at];
-  W* out = static_cast<W*>(at < c.width ? c.grad_weight : c.grad_bias);
-  if (out) out[at % c.width] = from_float<W>(sum);
+__global__ __launch_bounds__(256) void norm_backward_groups_kernel(odc_norm_backward c, uint32_t groups) {
+  __shared__ float scratch[16][kColumnTile];
+  const uint32_t part = threadIdx.x / 16, quad = threadIdx.x % 16 * 4;
+  const uint64_t at = (uint64_t)blockIdx.x * kColumnTile + quad, end = 2 * c.width;
+  const float* workspace = static_cast<const float*>(c.workspace);
+  float sum[4] = {};
+  if (at + 4 <= end) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll 4
+    for (uint32_t g = part; g < groups; g += 16) {
+      const f4 v = *reinterpret_cast<const f4*>(workspace + g * end + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+    }
+  } else {
+    for (uint32_t g = part; g < groups; g += 16)
+      for (int e = 0; e < 4; ++e)
+        if (at + e < end) sum[e] += workspace[g * end + at + e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) scratch[part][quad + e] = sum[e];
+  __syncthreads();
+  const uint64_t column = (uint64_t)blockIdx.x * kColumnTile + threadIdx.x;
+  if (threadIdx.x < kColumnTile && column < end) {
+    float all = scratch[0][threadIdx.x];
+#pragma unroll
+    for (int p = 1; p < 16; ++p) all += scratch[p][threadIdx.x];
+    W* out = static_cast<W*>(column < c.width ? c.grad_weight : c.grad_bias);
+    if (out) out[column < c.width ? column : column - c.width] = from_float<W>(all);
+  }
 }
 
+// ------------------------------------------------------------------------------------------------
+// launches
+// ------------------------------------------------------------------------------------------------
 // Calls body with a value of the element types' own.
 template <class Body>
 int with_types(int32_t dtype, int32_t weight_dtype, Body body) {
@@ -124,11 +420,36 @@ int with_types(int32_t dtype, int32_t weight_dtype, Body body) {
   return weight_dtype == ODC_OPS_F32 ? body(f16(), float()) : body(f16(), f16());
 }
 
+template <uint32_t n>
+struct Number {
+  static constexpr uint32_t value = n;
+};
+
+// Calls body with the shape's lanes and vectors as types; shapes[kAt] and those behind it.
+template <const auto& kShapes, size_t kAt = 0, class Body>
+void with_shape(NormShape shape, Body body) {
+  constexpr NormShape s = kShapes[kAt];
+  if (shape.lanes == s.lanes && shape.vectors == s.vectors) return body(Number<s.lanes>(), Number<s.vectors>());
+  if constexpr (kAt + 1 < sizeof(kShapes) / sizeof(NormShape)) with_shape<kShapes, kAt + 1>(shape, body);
+}
+
 }  // namespace
 
 int launch_norm_forward(const odc_norm_forward& call, const NormForwardPlan& plan, void* stream) {
   return with_types(call.dtype, call.weight_dtype, [&](auto t, auto w) {
-    norm_forward_kernel<decltype(t), decltype(w)><<<plan.blocks, kNormThreads, 0, (hipStream_t)stream>>>(call);
+    using T = decltype(t);
+    using W = decltype(w);
+    hipStream_t s = (hipStream_t)stream;
+    if (!plan.shape.lanes) {
+      norm_forward_wide_kernel<T, W><<<plan.blocks, kWideThreads, 0, s>>>(call);
+    } else {
+      with_shape<kForwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
+        constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
+        constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
+        if (call.residual) norm_forward_kernel<T, W, kLanes, kVectors, true><<<plan.blocks, kThreads, 0, s>>>(call);
+        else norm_forward_kernel<T, W, kLanes, kVectors, false><<<plan.blocks, kThreads, 0, s>>>(call);
+      });
+    }
     return (int)hipGetLastError();
   });
 }
@@ -138,12 +459,19 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
     using T = decltype(t);
     using W = decltype(w);
     hipStream_t s = (hipStream_t)stream;
-    if (call.rows && call.grad_input) norm_backward_rows_kernel<T, W><<<plan.row_blocks, kNormThreads, 0, s>>>(call);
-    if (call.grad_weight || call.grad_bias) {
+    const bool sums = call.grad_weight || call.grad_bias;
+    if (plan.shape.lanes && plan.groups) {
+      with_shape<kBackwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
+        norm_backward_kernel<T, W, (int)decltype(lanes)::value, (int)decltype(vectors)::value><<<plan.groups, kBackwardThreads, 0, s>>>(call);
+      });
+    } else if (plan.groups) {
+      if (call.grad_input) norm_backward_rows_kernel<T, W><<<plan.row_blocks, kWideThreads, 0, s>>>(call);
       const uint32_t tiles = (uint32_t)((call.width + kColumnTile - 1) / kColumnTile);
-      if (plan.groups) norm_backward_columns_kernel<T><<<dim3(tiles, plan.groups), kNormThreads, 0, s>>>(call, plan.rows_per_group);
-      const uint32_t blocks = (uint32_t)((2 * call.width + kNormThreads - 1) / kNormThreads);
-      norm_backward_groups_kernel<W><<<blocks, kNormThreads, 0, s>>>(call, plan.groups);
+      if (sums) norm_backward_columns_kernel<T><<<dim3(tiles, plan.groups), kWideThreads, 0, s>>>(call, plan.rows_per_group);
+    }
+    if (sums) {
+      const uint32_t blocks = (uint32_t)((2 * call.width + kColumnTile - 1) / kColumnTile);
+      norm_backward_groups_kernel<W><<<blocks, 256, 0, s>>>(call, plan.groups);
     }
     return (int)hipGetLastError();
   });

@@ -59,11 +59,32 @@ int check_rows(const char* name, const void* p, uint64_t rows, uint64_t width, u
     if (rc_ != ODC_OPS_OK) return rc_;             \
   } while (0)
 
-NormBackwardPlan backward_plan(uint64_t rows, uint64_t) {
+constexpr uint64_t kCus = 256;
+
+NormForwardPlan forward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
+  NormForwardPlan plan;
+  plan.shape = shape_of(kForwardShapes, width, dtype);
+  uint64_t rows_at_once = 1, most = 8 * kCus;
+  if (plan.shape.lanes) {
+    const uint32_t threads = std::max(kForwardThreads, plan.shape.lanes);
+    rows_at_once = threads / plan.shape.lanes;
+    most = 2048 / threads * kCus;
+  }
+  plan.blocks = (uint32_t)std::min(ceil_div(rows, rows_at_once), most);
+  return plan;
+}
+
+NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
   NormBackwardPlan plan;
-  plan.row_blocks = (uint32_t)std::min<uint64_t>(rows, 1u << 20);
-  plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kMostGroups));
-  plan.groups = (uint32_t)ceil_div(rows, plan.rows_per_group);
+  plan.shape = shape_of(kBackwardShapes, width, dtype);
+  plan.row_blocks = (uint32_t)std::min<uint64_t>(rows, 8 * kCus);
+  if (plan.shape.lanes) {
+    plan.groups = (uint32_t)std::min(ceil_div(rows, kBackwardThreads / plan.shape.lanes), kCus);
+    plan.rows_per_group = 0;
+  } else {
+    plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kCus));
+    plan.groups = (uint32_t)ceil_div(rows, plan.rows_per_group);
+  }
   return plan;
 }
 
@@ -110,12 +131,12 @@ int odc_layer_norm(const odc_norm_forward* call, void* stream) {
   ODC_OPS_TRY(check_rows("weight", c.weight, 1, c.width, c.width, c.weight_dtype, false));
   ODC_OPS_TRY(check_rows("bias", c.bias, 1, c.width, c.width, c.weight_dtype, false));
   if (!aligned(c.mean, 4) || !aligned(c.rstd, 4)) return fail(ODC_OPS_ERR_INVALID, "mean or rstd is not aligned to its element");
-  return launched(odc_ops_device::launch_norm_forward(c, {(uint32_t)std::min<uint64_t>(c.rows, 1u << 20)}, stream));
+  return launched(odc_ops_device::launch_norm_forward(c, forward_plan(c.rows, c.width, c.dtype), stream));
 }
 
 uint64_t odc_layer_norm_backward_workspace(uint64_t rows, uint64_t width, int32_t dtype) {
   if (check_norm(rows, width, dtype, ODC_OPS_F32) != ODC_OPS_OK || !rows || !width) return 0;
-  return (uint64_t)backward_plan(rows, width).groups * 2 * width * sizeof(float);
+  return (uint64_t)backward_plan(rows, width, dtype).groups * 2 * width * sizeof(float);
 }
 
 int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {
@@ -138,7 +159,7 @@ int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {
     if (need && (!c.workspace || c.workspace_bytes < need)) return fail(ODC_OPS_ERR_INVALID, "the workspace needs %llu bytes", (unsigned long long)need);
     if (!aligned(c.workspace, 16)) return fail(ODC_OPS_ERR_INVALID, "the workspace is not aligned to 16 bytes");
   }
-  return launched(odc_ops_device::launch_norm_backward(c, backward_plan(c.rows, c.width), stream));
+  return launched(odc_ops_device::launch_norm_backward(c, backward_plan(c.rows, c.width, c.dtype), stream));
 }
 
 uint64_t odc_squared_norm_workspace(const odc_span_item* items, uint32_t n_items, int32_t dtype) {

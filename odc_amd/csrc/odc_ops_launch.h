@@ -6,6 +6,7 @@
 #ifndef ODC_OPS_LAUNCH_H_
 #define ODC_OPS_LAUNCH_H_
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include "odc_ops.h"
@@ -16,21 +17,39 @@ inline bool is_float_type(int32_t dtype) { return dtype == ODC_OPS_BF16 || dtype
 inline uint32_t bytes_of(int32_t dtype) { return dtype == ODC_OPS_F32 ? 4 : 2; }
 
 // ---- layer norm -----------------------------------------------------------------------------------
-constexpr uint32_t kNormThreads = 256;
-// The gradients of weight and bias are sums over the rows. `groups` workgroups add up rows of their own, each
-// into its row of the workspace ([groups][2][width] floats), and a second launch adds the groups.
-constexpr uint32_t kColumnTile = 64;  // columns of one workgroup of the column sums
-constexpr uint32_t kMostGroups = 256;
+// A row is held in the registers of `lanes` lanes, `vectors` vectors of 16 bytes each; rows wider than the last shape
+// are passed over three times.
+struct NormShape {
+  uint32_t lanes, vectors;
+};
+constexpr NormShape kForwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}, {1024, 4}};
+constexpr NormShape kBackwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}};
+constexpr uint32_t kForwardThreads = 256;    // of a workgroup; where a row takes more lanes, as many as those
+constexpr uint32_t kBackwardThreads = 1024;
+constexpr uint32_t kWideThreads = 256;       // of one for wide rows
+
+// The first of `shapes` that holds a row; lanes 0: none does.
+template <size_t n>
+inline NormShape shape_of(const NormShape (&shapes)[n], uint64_t width, int32_t dtype) {
+  for (const NormShape& s : shapes)
+    if (width <= (uint64_t)s.lanes * s.vectors * (16 / bytes_of(dtype))) return s;
+  return {0, 0};
+}
 
 struct NormForwardPlan {
+  NormShape shape;
   uint32_t blocks;
 };
 
+// The gradients of weight and bias are sums over the rows. `groups` workgroups add up rows of their own, each
+// into its row of the workspace ([groups][2][width] floats), and a second launch adds the groups.
 struct NormBackwardPlan {
-  uint32_t row_blocks;  // workgroups of the pass over rows
+  NormShape shape;
   uint32_t groups;
-  uint64_t rows_per_group;
+  uint32_t row_blocks;      // wide rows: workgroups of the pass over rows
+  uint64_t rows_per_group;  // wide rows: of the pass over columns
 };
+constexpr uint32_t kColumnTile = 64;  // columns of one workgroup of the passes over columns
 
 // ---- lists of tensors -----------------------------------------------------------------------------
 // A dispatch counts its work-items in 32 bits: the most workgroups of 256.
