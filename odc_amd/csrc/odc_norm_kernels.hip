@@ -10,14 +10,23 @@ using namespace odc_ops_launch;
 // ------------------------------------------------------------------------------------------------
 // rows in registers
 // ------------------------------------------------------------------------------------------------
-// kElems neighbouring elements of a row from element i on; what lies behind the row's end is zero, and not read.
-template <int kElems, class T>
+// kElems neighbouring elements of a row from element i on; what lies behind the row's end is zero, and neither read
+// nor written. kBuffer: rows start at multiples of 16 bytes and end with a whole piece, and all lanes agree on the
+// row. It is then a buffer of its own to the hardware, whose bounds check takes the place of branches around the
+// accesses (which had cost the backward pass 20 registers).
+template <int kElems, class T, bool kBuffer>
 struct Piece {
   static constexpr int kVectors = kElems / Vector<T>::kElems;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   typename Vector<T>::type v[kVectors];
 
   __device__ __forceinline__ void load(const T* row, uint32_t i, uint32_t width) {
-    if (i + kElems <= width) {
+    if constexpr (kBuffer) {
+      const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, width * sizeof(T), 0x00027000);
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k)
+        v[k] = __builtin_bit_cast(typename Vector<T>::type, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(buffer, i * sizeof(T) + k * 16, 0, 0));
+    } else if (i + kElems <= width) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) v[k] = *reinterpret_cast<const typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems);
     } else {
@@ -26,7 +35,12 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void store(T* row, uint32_t i, uint32_t width) const {
-    if (i + kElems <= width) {
+    if constexpr (kBuffer) {
+      const auto buffer = __builtin_amdgcn_make_buffer_rsrc(row, 0, width * sizeof(T), 0x00027000);
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), buffer, i * sizeof(T) + k * 16, 0, 0);
+    } else if (i + kElems <= width) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) *reinterpret_cast<typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems) = v[k];
     } else {
@@ -40,11 +54,18 @@ struct Piece {
   // What was computed from it so far is forgotten: the compiler would keep the converted values over a barrier, in
   // twice the registers, where converting them again costs an instruction each.
   __device__ __forceinline__ void forget() {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) asm("" : "+v"(reinterpret_cast<u32x4&>(v[k])));
   }
 };
+
+// Which of a workgroup's rows a thread works on: the same for all of a wavefront where a row takes one or more, which
+// keeps the rows' addresses in scalar registers.
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_slot() {
+  const uint32_t slot = threadIdx.x / kLanes;
+  return kLanes >= 64 ? __builtin_amdgcn_readfirstlane(slot) : slot;
+}
 
 // The sums of kValues values over the lanes of a row. More than a wavefront's meet in LDS: `scratch` has kValues floats
 // for every wavefront, and the caller alternates between two of them, so that one barrier is enough.
@@ -59,24 +80,21 @@ __device__ __forceinline__ void row_sums(float (&x)[kValues], float* scratch) {
       for (int v = 0; v < kValues; ++v) scratch[wave * kValues + v] = x[v];
     }
     __syncthreads();
-    const float* mine = scratch + wave / (kLanes / 64) * (kLanes / 64) * kValues;
+    constexpr int kWaves = kLanes / 64;  // neighbouring lanes take one wavefront's sums each
+    const float* mine = scratch + (wave / kWaves * kWaves + threadIdx.x % kWaves) * kValues;
 #pragma unroll
-    for (int v = 0; v < kValues; ++v) {
-      x[v] = mine[v];
-#pragma unroll
-      for (int w = 1; w < kLanes / 64; ++w) x[v] += mine[w * kValues + v];
-    }
+    for (int v = 0; v < kValues; ++v) x[v] = sum_lanes<kWaves>(mine[v]);
   }
 }
 
-template <class T, class W, int kLanes, int kVectors, bool kAdd>
+template <class T, class W, int kLanes, int kVectors, bool kBuffer, bool kAdd>
 __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads) void norm_forward_kernel(odc_norm_forward c) {
   constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
   constexpr int kElems = Vector<T>::kElems;
   __shared__ float scratch[2][kThreads / 64];
   const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes;
   const float per_element = 1.0f / (float)width;
-  Piece<kElems, W> weight[kVectors], bias[kVectors];
+  Piece<kElems, W, kBuffer> weight[kVectors], bias[kVectors];
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     const uint32_t i = (k * kLanes + lane) * kElems;
@@ -94,13 +112,13 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
     }
   }
   constexpr uint32_t kRows = kThreads / kLanes;  // at once
-  uint64_t row = (uint64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
-  Piece<kElems, T> x[kVectors], r[kVectors];
-  const auto load = [&](Piece<kElems, T>(&piece)[kVectors], const void* rows, uint64_t stride) {
+  uint64_t row = (uint64_t)blockIdx.x * kRows + row_slot<kLanes>();
+  Piece<kElems, T, kBuffer> x[kVectors], r[kVectors];
+  const auto load = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors], const void* rows, uint64_t stride) {
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows ? width : 0);
   };
-  const auto load_row = [&](Piece<kElems, T>(&piece)[kVectors]) {
+  const auto load_row = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors]) {
     load(piece, c.input, c.input_stride);
     if constexpr (kAdd) load(r, c.residual, c.residual_stride);
   };
@@ -122,7 +140,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 #pragma unroll
       for (int e = 0; e < kElems; ++e) sum[0] += x[k][e];
     const uint64_t here = row;
-    Piece<kElems, T> next[kVectors];
+    Piece<kElems, T, kBuffer> next[kVectors];
     row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
     if constexpr (kAhead) load_row(next);
     row_sums<kLanes>(sum, scratch[0]);
@@ -134,7 +152,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
     for (int k = 0; k < kVectors; ++k)
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
-        const float d = (k * kLanes + lane) * kElems + e < width ? x[k][e] - mean : 0.0f;
+        const float d = (k * kLanes + lane) * kElems + (kBuffer ? 0 : e) < width ? x[k][e] - mean : 0.0f;
         squares[0] += d * d;
       }
     row_sums<kLanes>(squares, scratch[1]);
@@ -157,37 +175,50 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 // A workgroup passes over rows blockIdx.x, + gridDim.x, ... (kThreads / kLanes of them at once), writes their
 // grad_input and keeps the sums for weight and bias of its lanes' columns in registers; at the end the rows that it had
 // at once are added in LDS, upper half onto lower half, and go to its row of the workspace.
-template <class T, class W, int kLanes, int kVectors>
-__global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_norm_backward c) {
-  constexpr int kThreads = kBackwardThreads, kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
+template <class T, class W, int kLanes, int kVectors, bool kBuffer>
+__global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_backward_kernel(odc_norm_backward c) {
+  constexpr int kThreads = backward_threads({kLanes, kVectors}), kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
   constexpr int kSums = 2 * kVectors * kElems;  // of a thread
   __shared__ float scratch[2][2 * kThreads / 64];
   __shared__ float upper[kRows > 1 ? kThreads / 2 * kSums : 1];
-  const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes, slot = row_slot<kLanes>();
   const float per_element = 1.0f / (float)width;
   const bool sums = c.grad_weight || c.grad_bias;
-  Piece<kElems, W> weight[kVectors];
+  // The weights of a lane's columns stay in registers, or, where the sums and the rows need these, in LDS: every lane
+  // puts its own there.
+  constexpr bool kWeightInLds = kVectors > 1;
+  typedef Piece<kElems, W, kBuffer> Weight;
+  __shared__ typename Vector<W>::type weights[kWeightInLds ? kVectors * Weight::kVectors * kThreads : 1];
+  Weight weight_here[kWeightInLds ? 1 : kVectors];
   float dw[kVectors][kElems] = {}, db[kVectors][kElems] = {};
-  const auto load_weight = [&]() {
 #pragma unroll
-    for (int k = 0; k < kVectors; ++k) {
-      if (c.weight) {
-        weight[k].load(static_cast<const W*>(c.weight), (k * kLanes + lane) * kElems, width);
-      } else {
+  for (int k = 0; k < kVectors; ++k) {
+    Weight w;
+    if (c.weight) {
+      w.load(static_cast<const W*>(c.weight), (k * kLanes + lane) * kElems, width);
+    } else {
 #pragma unroll
-        for (int e = 0; e < kElems; ++e) weight[k].set(e, (W)1.0f);
-      }
+      for (int e = 0; e < kElems; ++e) w.set(e, (W)1.0f);
     }
+    if constexpr (kWeightInLds) {
+#pragma unroll
+      for (int v = 0; v < Weight::kVectors; ++v) weights[(k * Weight::kVectors + v) * kThreads + threadIdx.x] = w.v[v];
+    } else {
+      weight_here[k] = w;
+    }
+  }
+  const auto weight = [&](int k) {
+    if constexpr (!kWeightInLds) return weight_here[k];
+    Weight w;
+#pragma unroll
+    for (int v = 0; v < Weight::kVectors; ++v) w.v[v] = weights[(k * Weight::kVectors + v) * kThreads + threadIdx.x];
+    return w;
   };
-  // With one vector to a lane there are registers for the weights and for a row ahead; with two the weights are read
-  // again from the caches.
-  constexpr bool kAhead = kVectors == 1;
-  if constexpr (kAhead) load_weight();
   int parity = 0;
   uint64_t row = (uint64_t)blockIdx.x * kRows + slot;
-  Piece<kElems, T> x[kVectors], dy[kVectors], dt[kVectors];
+  Piece<kElems, T, kBuffer> x[kVectors], dy[kVectors], dt[kVectors];
   float mean, rstd;
-  const auto load = [&](Piece<kElems, T>(&piece)[kVectors], const void* rows, uint64_t stride) {
+  const auto load = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors], const void* rows, uint64_t stride) {
 #pragma unroll
     for (int k = 0; k < kVectors; ++k)
       piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows && rows ? width : 0);
@@ -198,48 +229,51 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_nor
     mean = row < c.rows ? c.mean[row] : 0;
     rstd = row < c.rows ? c.rstd[row] : 0;
   };
+  // Where registers allow, the next row is on its way while this one's sums are made.
+  constexpr bool kAhead = kBuffer || kVectors == 1;
   if constexpr (kAhead) load_row();
   // every thread makes the same number of rounds: there are barriers in them
   for (uint64_t first = (uint64_t)blockIdx.x * kRows; first < c.rows; first += (uint64_t)gridDim.x * kRows, parity ^= 1) {
-    if constexpr (!kAhead) {
-      load_row();
-      load_weight();
-    }
-    if (c.grad_input) load(dt, c.grad_total, c.grad_total_stride);
+    if constexpr (!kAhead) load_row();
     float row_sum[2] = {};
 #pragma unroll
-    for (int k = 0; k < kVectors; ++k)
+    for (int k = 0; k < kVectors; ++k) {
+      const Weight w = weight(k);
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
         const float z = (x[k][e] - mean) * rstd, g = dy[k][e];  // behind the row's end g is zero and z of no account
-        const float h = g * weight[k][e];
+        const float h = g * w[e];
         row_sum[0] += h;
         row_sum[1] += h * z;
         dw[k][e] += g * z;
         db[k][e] += g;
       }
+      if constexpr (kVectors > 1) __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time: registers
+    }
     const uint64_t here = row;
     const float mean_here = mean, rstd_here = rstd;
-    Piece<kElems, T> x_here[kVectors], dy_here[kVectors];
+    Piece<kElems, T, kBuffer> x_here[kVectors], dy_here[kVectors];
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) x_here[k] = x[k], dy_here[k] = dy[k];
-    row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
+    if (c.grad_input) load(dt, c.grad_total, c.grad_total_stride);
+    row += (uint64_t)gridDim.x * kRows;
     if constexpr (kAhead) load_row();
     if (c.grad_input) {
       row_sums<kLanes>(row_sum, scratch[parity]);
       const float sum = row_sum[0] * per_element, dot = row_sum[1] * per_element;
       if (here < c.rows) {
-        if constexpr (!kAhead) load_weight();
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
           x_here[k].forget();
           dy_here[k].forget();
+          const Weight w = weight(k);
 #pragma unroll
           for (int e = 0; e < kElems; ++e) {
-            const float z = (x_here[k][e] - mean_here) * rstd_here, h = dy_here[k][e] * weight[k][e];
+            const float z = (x_here[k][e] - mean_here) * rstd_here, h = dy_here[k][e] * w[e];
             x_here[k].set(e, from_float<T>(rstd_here * (h - sum - z * dot) + dt[k][e]));
           }
           x_here[k].store(static_cast<T*>(c.grad_input) + here * c.width, (k * kLanes + lane) * kElems, width);
+          if constexpr (kVectors > 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -433,6 +467,19 @@ void with_shape(NormShape shape, Body body) {
   if constexpr (kAt + 1 < sizeof(kShapes) / sizeof(NormShape)) with_shape<kShapes, kAt + 1>(shape, body);
 }
 
+template <class Body>
+void with_truth(bool truth, Body body) {
+  if (truth) body(Number<1>());
+  else body(Number<0>());
+}
+
+// Rows that share a wavefront are no buffers (the plan does not ask for it).
+template <int kLanes, class Body>
+void with_buffers(bool buffers, Body body) {
+  if constexpr (kLanes >= 64) with_truth(buffers, body);
+  else body(Number<0>());
+}
+
 }  // namespace
 
 int launch_norm_forward(const odc_norm_forward& call, const NormForwardPlan& plan, void* stream) {
@@ -446,8 +493,11 @@ int launch_norm_forward(const odc_norm_forward& call, const NormForwardPlan& pla
       with_shape<kForwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
         constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
         constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
-        if (call.residual) norm_forward_kernel<T, W, kLanes, kVectors, true><<<plan.blocks, kThreads, 0, s>>>(call);
-        else norm_forward_kernel<T, W, kLanes, kVectors, false><<<plan.blocks, kThreads, 0, s>>>(call);
+        with_buffers<kLanes>(plan.buffers, [&](auto buffers) {
+          with_truth(call.residual != nullptr, [&](auto add) {
+            norm_forward_kernel<T, W, kLanes, kVectors, decltype(buffers)::value, decltype(add)::value><<<plan.blocks, kThreads, 0, s>>>(call);
+          });
+        });
       });
     }
     return (int)hipGetLastError();
@@ -462,7 +512,10 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
     const bool sums = call.grad_weight || call.grad_bias;
     if (plan.shape.lanes && plan.groups) {
       with_shape<kBackwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
-        norm_backward_kernel<T, W, (int)decltype(lanes)::value, (int)decltype(vectors)::value><<<plan.groups, kBackwardThreads, 0, s>>>(call);
+        constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
+        with_buffers<kLanes>(plan.buffers, [&](auto buffers) {
+          norm_backward_kernel<T, W, kLanes, kVectors, decltype(buffers)::value><<<plan.groups, backward_threads(plan.shape), 0, s>>>(call);
+        });
       });
     } else if (plan.groups) {
       if (call.grad_input) norm_backward_rows_kernel<T, W><<<plan.row_blocks, kWideThreads, 0, s>>>(call);

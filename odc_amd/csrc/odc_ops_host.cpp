@@ -61,8 +61,23 @@ int check_rows(const char* name, const void* p, uint64_t rows, uint64_t width, u
 
 constexpr uint64_t kCus = 256;
 
+// Whether rows of whole 16 byte vectors start at multiples of 16 bytes. (A wavefront has one row or a part of one then:
+// kLanes is 64 at least.)
+bool rows_of_vectors(const void* p, uint64_t stride, int32_t dtype) { return aligned(p, 16) && stride * bytes_of(dtype) % 16 == 0; }
+
+bool buffers(const odc_norm_forward& c, const NormShape& shape) {
+  return shape.lanes >= 64 && rows_of_vectors(c.input, c.input_stride, c.dtype) && rows_of_vectors(c.residual, c.residual_stride, c.dtype) &&
+         rows_of_vectors(c.output, c.width, c.dtype) && rows_of_vectors(c.total, c.width, c.dtype) && aligned(c.weight, 16) && aligned(c.bias, 16);
+}
+
+bool buffers(const odc_norm_backward& c, const NormShape& shape) {
+  return shape.lanes >= 64 && rows_of_vectors(c.grad_output, c.grad_output_stride, c.dtype) &&
+         rows_of_vectors(c.grad_total, c.grad_total_stride, c.dtype) && rows_of_vectors(c.normalised, c.normalised_stride, c.dtype) &&
+         c.width * bytes_of(c.dtype) % 16 == 0 && aligned(c.grad_input, 16) && aligned(c.weight, 16);
+}
+
 NormForwardPlan forward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
-  NormForwardPlan plan;
+  NormForwardPlan plan = {};
   plan.shape = shape_of(kForwardShapes, width, dtype);
   uint64_t rows_at_once = 1, most = 8 * kCus;
   if (plan.shape.lanes) {
@@ -75,11 +90,11 @@ NormForwardPlan forward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
 }
 
 NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
-  NormBackwardPlan plan;
+  NormBackwardPlan plan = {};
   plan.shape = shape_of(kBackwardShapes, width, dtype);
   plan.row_blocks = (uint32_t)std::min<uint64_t>(rows, 8 * kCus);
   if (plan.shape.lanes) {
-    plan.groups = (uint32_t)std::min(ceil_div(rows, kBackwardThreads / plan.shape.lanes), kCus);
+    plan.groups = (uint32_t)std::min(ceil_div(rows, backward_threads(plan.shape) / plan.shape.lanes), kCus);
     plan.rows_per_group = 0;
   } else {
     plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kCus));
@@ -131,7 +146,9 @@ int odc_layer_norm(const odc_norm_forward* call, void* stream) {
   ODC_OPS_TRY(check_rows("weight", c.weight, 1, c.width, c.width, c.weight_dtype, false));
   ODC_OPS_TRY(check_rows("bias", c.bias, 1, c.width, c.width, c.weight_dtype, false));
   if (!aligned(c.mean, 4) || !aligned(c.rstd, 4)) return fail(ODC_OPS_ERR_INVALID, "mean or rstd is not aligned to its element");
-  return launched(odc_ops_device::launch_norm_forward(c, forward_plan(c.rows, c.width, c.dtype), stream));
+  NormForwardPlan plan = forward_plan(c.rows, c.width, c.dtype);
+  plan.buffers = buffers(c, plan.shape);
+  return launched(odc_ops_device::launch_norm_forward(c, plan, stream));
 }
 
 uint64_t odc_layer_norm_backward_workspace(uint64_t rows, uint64_t width, int32_t dtype) {
@@ -159,7 +176,9 @@ int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {
     if (need && (!c.workspace || c.workspace_bytes < need)) return fail(ODC_OPS_ERR_INVALID, "the workspace needs %llu bytes", (unsigned long long)need);
     if (!aligned(c.workspace, 16)) return fail(ODC_OPS_ERR_INVALID, "the workspace is not aligned to 16 bytes");
   }
-  return launched(odc_ops_device::launch_norm_backward(c, backward_plan(c.rows, c.width, c.dtype), stream));
+  NormBackwardPlan plan = backward_plan(c.rows, c.width, c.dtype);
+  plan.buffers = buffers(c, plan.shape);
+  return launched(odc_ops_device::launch_norm_backward(c, plan, stream));
 }
 
 uint64_t odc_squared_norm_workspace(const odc_span_item* items, uint32_t n_items, int32_t dtype) {

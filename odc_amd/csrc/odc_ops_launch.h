@@ -25,7 +25,7 @@ struct NormShape {
 constexpr NormShape kForwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}, {1024, 4}};
 constexpr NormShape kBackwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}};
 constexpr uint32_t kForwardThreads = 256;    // of a workgroup; where a row takes more lanes, as many as those
-constexpr uint32_t kBackwardThreads = 1024;
+constexpr uint32_t backward_threads(NormShape) { return 1024; }
 constexpr uint32_t kWideThreads = 256;       // of one for wide rows
 
 // The first of `shapes` that holds a row; lanes 0: none does.
@@ -38,6 +38,7 @@ inline NormShape shape_of(const NormShape (&shapes)[n], uint64_t width, int32_t 
 
 struct NormForwardPlan {
   NormShape shape;
+  bool buffers;  // every row is a buffer of whole vectors (Piece in odc_norm_kernels.hip)
   uint32_t blocks;
 };
 
@@ -45,6 +46,7 @@ struct NormForwardPlan {
 // into its row of the workspace ([groups][2][width] floats), and a second launch adds the groups.
 struct NormBackwardPlan {
   NormShape shape;
+  bool buffers;
   uint32_t groups;
   uint32_t row_blocks;      // wide rows: workgroups of the pass over rows
   uint64_t rows_per_group;  // wide rows: of the pass over columns
