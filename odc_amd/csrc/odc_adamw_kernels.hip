@@ -1,4 +1,6 @@
 // odc_adamw_kernels.hip — the squared norm and the AdamW step of many tensors for gfx950.
+#include <type_traits>
+
 #include "odc_ops_device.h"
 #include "odc_ops_launch.h"
 
@@ -8,27 +10,58 @@ namespace {
 using namespace odc_ops_launch;
 
 // ---- squared norm ---------------------------------------------------------------------------------
-template <class T>
+// Every lane adds up the 32 squares that it has of a tile in fp32, the tiles in 64 bits.
+template <class T, bool kStream>
 __global__ __launch_bounds__(256) void squared_norm_kernel(SquaredNormLaunch launch, double* partials) {
+  constexpr uint32_t kElems = Vector<T>::kElems, kSteps = kNormTile / (256 * kElems);
   __shared__ double scratch[4];
-  float sum = 0;
+  double total = 0;
   for (uint32_t tile = blockIdx.x; tile < launch.n_tiles; tile += gridDim.x) {
     const uint32_t k = item_of(launch, tile);
-    const T* data = static_cast<const T*>(launch.items[k].data);
-    const uint64_t first = (uint64_t)(tile - launch.first_tile[k]) * kNormTile;
-    const uint64_t end = first + kNormTile < launch.items[k].elems ? first + kNormTile : launch.items[k].elems;
-    for (uint64_t i = first + threadIdx.x; i < end; i += 256) {
-      const float x = to_float(data[i]);
-      sum += x * x;
+    const uint64_t first = (uint64_t)(tile - launch.first_tile[k]) * kNormTile, left = launch.items[k].elems - first;
+    const T* data = static_cast<const T*>(launch.items[k].data) + first;
+    float sum[kElems] = {};
+    if (left >= kNormTile) {
+      typename Vector<T>::type x[kSteps];
+#pragma unroll
+      for (uint32_t s = 0; s < kSteps; ++s) {
+        const auto* p = reinterpret_cast<const typename Vector<T>::unaligned*>(data + (s * 256 + threadIdx.x) * kElems);
+        if constexpr (kStream) x[s] = __builtin_nontemporal_load(p);
+        else x[s] = *p;
+      }
+#pragma unroll
+      for (uint32_t s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (uint32_t e = 0; e < kElems; ++e) sum[e] += to_float(x[s][e]) * to_float(x[s][e]);
+    } else {
+      for (uint32_t i = threadIdx.x * kElems; i < left; i += 256 * kElems) {
+        if (i + kElems <= left) {
+          const typename Vector<T>::type x = *reinterpret_cast<const typename Vector<T>::unaligned*>(data + i);
+#pragma unroll
+          for (uint32_t e = 0; e < kElems; ++e) sum[e] += to_float(x[e]) * to_float(x[e]);
+        } else {
+#pragma unroll
+          for (uint32_t e = 0; e < kElems; ++e) {
+            const float x = i + e < left ? to_float(data[i + e]) : 0.0f;
+            sum[e] += x * x;
+          }
+        }
+      }
     }
+#pragma unroll
+    for (uint32_t width = kElems / 2; width; width /= 2)
+#pragma unroll
+      for (uint32_t e = 0; e < width; ++e) sum[e] += sum[e + width];
+    total += sum[0];
   }
-  const double all = block_sum<256>((double)sum, scratch);
-  if (threadIdx.x == 0) partials[blockIdx.x] = all;
+  total = block_sum<256>(total, scratch);
+  if (threadIdx.x == 0) partials[blockIdx.x] = total;
 }
 
 __global__ __launch_bounds__(256) void squared_norm_total_kernel(const double* partials, uint32_t n, float* result) {
   __shared__ double scratch[4];
   double sum = 0;
+#pragma unroll 8
   for (uint32_t i = threadIdx.x; i < n; i += 256) sum += partials[i];
   sum = block_sum<256>(sum, scratch);
   if (threadIdx.x == 0) *result = (float)sum;
@@ -41,142 +74,285 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
+// The square root and the reciprocal of the hardware (1 ulp each), which take a subnormal number for zero. Only a v can be
+// one here: its root goes by root_of.
+__device__ __forceinline__ float fast_sqrt(float x) { return __builtin_amdgcn_sqrtf(x); }
+__device__ __forceinline__ float fast_reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
+
+__device__ __forceinline__ float root_of(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = fast_sqrt(small ? v * 0x1p32f : v);
+  return small ? r * 0x1p-16f : r;
+}
+
 // The factor of the gradients. A norm that is not a number makes it not a number.
 __device__ __forceinline__ float factor_of(const AdamwLaunch& launch) {
   if (!launch.squared_norm) return launch.grad_scale;
-  const float c = launch.max_norm / (launch.grad_scale * sqrtf(*launch.squared_norm) + 1e-6f);
+  const float c = launch.max_norm * fast_reciprocal(launch.grad_scale * root_of(*launch.squared_norm) + 1e-6f);
   return launch.grad_scale * (c > 1.0f ? 1.0f : c);
 }
 
-struct Moments {
-  float m, v, root;
+// Four neighbouring elements, as a lane works on them: 16 bytes in fp32, so that a wavefront's accesses to every
+// list are whole lines. kStream: nontemporal. Only the first n of the four exist.
+template <class T>
+struct Four {
+  typedef T type __attribute__((ext_vector_type(4)));
+  typedef type unaligned __attribute__((aligned(sizeof(T))));
+  type v;
+
+  template <bool kStream>
+  __device__ __forceinline__ void load(const T* p, uint32_t n) {
+    if (n == 4) {
+      const auto* q = reinterpret_cast<const unaligned*>(p);
+      if constexpr (kStream) v = __builtin_nontemporal_load(q);
+      else v = *q;
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) v[e] = e < n ? p[e] : (T)0;
+    }
+  }
+  template <bool kStream>
+  __device__ __forceinline__ void store(T* p, uint32_t n) const {
+    if (n == 4) {
+      auto* q = reinterpret_cast<unaligned*>(p);
+      if constexpr (kStream) __builtin_nontemporal_store((unaligned)v, q);
+      else *q = v;
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 3; ++e)
+        if (e < n) p[e] = v[e];
+    }
+  }
 };
 
-__device__ __forceinline__ Moments next_moments(const AdamwLaunch& launch, float g, float m, float v) {
-  Moments out;
-  out.m = m * launch.beta1 + g * launch.one_minus_beta1;
-  out.v = v * launch.beta2 + g * g * launch.one_minus_beta2;
-  out.root = sqrtf(out.v);
-  return out;
+// The roots of four values. Small ones are rare: a wavefront without any takes the instruction as it is.
+__device__ __forceinline__ void roots_of(const float (&v)[4], float (&root)[4]) {
+  const float least = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+  if (__ballot(least < 0x1p-96f)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) root[e] = root_of(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) root[e] = fast_sqrt(v[e]);
+  }
 }
 
-__device__ __forceinline__ float next_param(const AdamwLaunch& launch, float p, const Moments& s) {
-  return p * launch.decay - launch.step_size * (s.m / (s.root * launch.root_scale + launch.eps));
+// (The denominator is no subnormal number: the root of the smallest v above zero is 3.7e-23.)
+__device__ __forceinline__ float next_param(const AdamwLaunch& launch, float p, float m, float root) {
+  return p * launch.decay - launch.step_size * (m * fast_reciprocal(root * launch.root_scale + launch.eps));
 }
 
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+
+// A parameter as it is stored: in bf16 by its random bits, if there are any.
+template <class P>
+__device__ __forceinline__ P stored_param(float p, bool stochastic, uint32_t word) {
+  if constexpr (sizeof(P) == 2) {
+    if (stochastic && is_finite(p)) return from_float<P>(__uint_as_float((__float_as_uint(p) + (mix(word ^ 0x5BF03635u) & 0xFFFFu)) & 0xFFFF0000u));
+  }
+  return from_float<P>(p);
+}
+
+__device__ __forceinline__ uint32_t word_of(uint64_t i, uint32_t key) { return mix((uint32_t)i + (uint32_t)(i >> 32) * 0x632BE5ABu + key); }
+
+// ---- states in 8 bits -----------------------------------------------------------------------------
 // The biased exponent of a block's scale from its largest value: the smallest power of two that keeps it
 // within 448 = 1.75 * 2^8.
-__device__ __forceinline__ uint32_t scale_of(float largest) {
-  const int k = (int)((__float_as_uint(largest) + 0x1FFFFFu) >> 23) - 8;
+__device__ __forceinline__ uint32_t scale_of(uint32_t largest_bits) {
+  const int k = (int)((largest_bits + 0x1FFFFFu) >> 23) - 8;
   return k < 10 ? 10u : (uint32_t)k;
 }
 
-// The e4m3 value beside |x| / scale that the 16 bits of `chance` choose, as code; x's sign with it. kSquares:
-// the expectation of the square is kept.
-template <bool kSquares>
-__device__ __forceinline__ uint32_t code_of(float x, uint32_t scale, uint32_t chance) {
-  if (!(fabsf(x) < INFINITY)) return 0x7F;
-  float size = fabsf(x) * __uint_as_float((254u - scale) << 23);
-  if (kSquares && size > 0) size = fmaxf(size, 0x1p-9f);
-  const float step = __uint_as_float(__float_as_uint(fmaxf(size, 0x1p-6f)) & 0x7F800000u) * 0.125f;
-  const float below = floorf(size / step) * step;
-  float share = size - below, whole = step;
-  if (kSquares) {
-    share *= size + below;
-    whole *= below + below + step;
-  }
-  const float chosen = ((float)chance + 0.5f) * whole < share * 65536.0f ? below + step : below;
-  const uint32_t pair = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(copysignf(chosen, x), 0.0f, 0, false);
-  return pair & 0xFF;
-}
-
-__device__ __forceinline__ float value_of(uint32_t code, uint32_t scale) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * __uint_as_float(scale << 23);
-}
-
-template <class P, class G, class C>
-__global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(AdamwLaunch launch) {
-  const uint32_t k = item_of(launch, blockIdx.x);
-  const odc_adamw_item& it = launch.items[k];
-  const float factor = factor_of(launch);
-  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kAdamwTile;
-  for (uint32_t j = threadIdx.x; j < kAdamwTile; j += kAdamwThreads) {
-    const uint64_t i = first + j;
-    if (i >= it.elems) break;
-    const float g = to_float(static_cast<const G*>(it.grad)[i]) * factor;
-    float* m = static_cast<float*>(it.exp_avg) + i;
-    float* v = static_cast<float*>(it.exp_avg_sq) + i;
-    P* param = static_cast<P*>(it.param) + i;
-    const Moments s = next_moments(launch, g, *m, *v);
-    *m = s.m;
-    *v = s.v;
-    const float p = next_param(launch, to_float(*param), s);
-    if (sizeof(P) == 2 && launch.stochastic) {
-      const uint64_t n = i;
-      const uint32_t word = mix((uint32_t)n + (uint32_t)(n >> 32) * 0x632BE5ABu + mix(launch.seed + (launch.first_item + k) * 0x9E3779B1u));
-      uint32_t bits = __float_as_uint(p);
-      if (fabsf(p) < INFINITY) bits = (bits + (mix(word ^ 0x5BF03635u) & 0xFFFFu)) & 0xFFFF0000u;
-      *param = from_float<P>(__uint_as_float(bits));
-    } else {
-      *param = from_float<P>(p);
-    }
-    if (it.copy) static_cast<C*>(it.copy)[i] = from_float<C>(p);
-  }
-}
-
-// A block of 32 elements is half a wavefront, whose lanes all come along.
-template <class P, class G, class C>
-__global__ __launch_bounds__(kAdamwThreads) void adamw8_kernel(AdamwLaunch launch) {
-  const uint32_t k = item_of(launch, blockIdx.x);
-  const odc_adamw_item& it = launch.items[k];
-  const float factor = factor_of(launch);
-  const uint32_t key = mix(launch.seed + (launch.first_item + k) * 0x9E3779B1u);
-  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kAdamwTile;
-  uint8_t* codes_m = static_cast<uint8_t*>(it.exp_avg);
-  uint8_t* codes_v = static_cast<uint8_t*>(it.exp_avg_sq);
-  uint8_t* scales_m = static_cast<uint8_t*>(it.exp_avg_scale);
-  uint8_t* scales_v = static_cast<uint8_t*>(it.exp_avg_sq_scale);
-  for (uint32_t j = threadIdx.x; j < kAdamwTile; j += kAdamwThreads) {
-    const uint64_t i = first + j, block = i / kBlock;
-    const bool mine = i < it.elems;
-    Moments s = {0, 0, 0};
-    P* param = static_cast<P*>(it.param) + i;
-    if (mine) {
-      const float g = to_float(static_cast<const G*>(it.grad)[i]) * factor;
-      const float root = value_of(codes_v[i], scales_v[block]);
-      s = next_moments(launch, g, value_of(codes_m[i], scales_m[block]), root * root);
-    }
-    float top_m = fabsf(s.m) < INFINITY ? fabsf(s.m) : 0, top_v = s.root < INFINITY ? s.root : 0;
+// The largest magnitude of a block, as bits, from the four values of each of its 8 lanes. As whole numbers the bits
+// are ordered as the magnitudes are, with what is not finite on top: that counts for nothing here, and `odd` says
+// whether any lane of the wavefront has it.
+__device__ __forceinline__ uint32_t largest_of(const float (&x)[4], bool& odd) {
+  const auto over_lanes = [](uint32_t top) {
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, top, 0xB1, 0xf, 0xf, true));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, top, 0x4E, 0xf, 0xf, true));
+    return max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, top, 0x141, 0xf, 0xf, true));
+  };
+  uint32_t top = 0;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      top_m = fmaxf(top_m, __shfl_xor(top_m, d));
-      top_v = fmaxf(top_v, __shfl_xor(top_v, d));
+  for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(x[e])));
+  const uint32_t all = over_lanes(top);
+  odd = __ballot(all >= 0x7F800000u) != 0;
+  if (!odd) return all;
+  top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, is_finite(x[e]) ? __float_as_uint(fabsf(x[e])) : 0u);
+  return over_lanes(top);
+}
+
+// The e4m3 value, as a float, beside |x| / 2^(scale - 127) that the 16 bits of `half` choose: the upper one where
+// (half + 0.5) / 65536 is less than the share of the way. Below 2^-6 the codes lie 2^-9 apart, as they do in the
+// binade above: 2^-6 is added there and taken away again.
+//
+// Where the expectation of the value is kept, the choice is an addition: 20 bits of the mantissa lie below a code's
+// three, and they reach the code above where they and what is added make 2^20.
+__device__ __forceinline__ float chosen_value(float x, float inverse_scale, uint32_t half) {
+  const float size = fabsf(x) * inverse_scale;
+  const float shift = size < 0x1p-6f ? 0x1p-6f : 0.0f;
+  const uint32_t bits = __float_as_uint(size + shift) + (0x100000u - 9) - half * 16;
+  return __uint_as_float(bits & 0xFFF00000u) - shift;
+}
+
+// Where that of the square is kept: with the codes a and a + s beside t the share is (t - a)(t + a) / (s (2 a + s)).
+// What is not zero does not become zero. `eight` is 8 s, the power of two that t begins with.
+__device__ __forceinline__ float chosen_root(float x, float inverse_scale, uint32_t half) {
+  float size = x * inverse_scale;
+  size = size > 0 ? fmaxf(size, 0x1p-9f) : size;
+  const float shift = size < 0x1p-6f ? 0x1p-6f : 0.0f;
+  const float lifted = size + shift;
+  const uint32_t bits = __float_as_uint(lifted);
+  const float below_lifted = __uint_as_float(bits & 0xFFF00000u), eight = __uint_as_float(bits & 0x7F800000u);
+  const float below = below_lifted - shift;
+  const float whole = ((float)half * 0x1p-22f + 0x1p-23f) * eight * (16 * below + eight);  // 64 times s (2 a + s), in 2^-16
+  return whole < (lifted - below_lifted) * (size + below) ? below + 0.125f * eight : below;
+}
+
+__device__ __forceinline__ float scale_value(uint32_t scale) { return __uint_as_float(scale << 23); }
+
+// Four codes as values, times `factor`.
+__device__ __forceinline__ void values_of(uint32_t codes, float factor, float (&x)[4]) {
+  x[0] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 0) * factor;
+  x[1] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 1) * factor;
+  x[2] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 2) * factor;
+  x[3] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 3) * factor;
+}
+
+// The codes of four values and the scale of their block. kRoots: roots, by the high halves of the words; else by the
+// low ones.
+template <bool kRoots>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], const uint32_t (&word)[4], uint32_t& scale) {
+  bool odd;
+  scale = scale_of(largest_of(x, odd));
+  const float inverse = __uint_as_float((254u - scale) << 23);
+  float c[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c[e] = kRoots ? chosen_root(x[e], inverse, word[e] >> 16) : copysignf(chosen_value(x[e], inverse, word[e] & 0xFFFFu), x[e]);
+  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+  uint32_t codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], low, true);
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!is_finite(x[e])) codes = (codes & ~(0xFFu << 8 * e)) | 0x7Fu << 8 * e;  // not a number
+  }
+  return codes;
+}
+
+// ---- the step -------------------------------------------------------------------------------------
+// kVectors times four elements to a lane, all of their loads before the first store; `elems` from element `first` on.
+template <class P, class G, class C, bool kEight, bool kStream, bool kWhole>
+__device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k, uint64_t first, uint32_t elems) {
+  const odc_adamw_item& it = launch.items[k];
+  constexpr AdamwShape kShape = adamw_shape(kEight);
+  constexpr uint32_t kThreads = kShape.threads, kVectors = kShape.vectors;
+  const float factor = factor_of(launch);
+  const bool stochastic = sizeof(P) == 2 && launch.stochastic;
+  const uint32_t key = kEight || stochastic ? mix(launch.seed + (launch.first_item + k) * 0x9E3779B1u) : 0;
+  P* const param = static_cast<P*>(it.param) + first;
+  const G* const grad = static_cast<const G*>(it.grad) + first;
+  C* const copy = it.copy ? static_cast<C*>(it.copy) + first : nullptr;
+  typedef std::conditional_t<kEight, uint8_t, float> S;
+  S* const m_state = static_cast<S*>(it.exp_avg) + first;
+  S* const v_state = static_cast<S*>(it.exp_avg_sq) + first;
+  uint8_t* const m_scale = static_cast<uint8_t*>(it.exp_avg_scale) + first / kBlock;
+  uint8_t* const v_scale = static_cast<uint8_t*>(it.exp_avg_sq_scale) + first / kBlock;
+  Four<P> p[kVectors];
+  Four<G> g[kVectors];
+  Four<S> m[kVectors], v[kVectors];
+  uint32_t m_exponent[kVectors], v_exponent[kVectors];
+#pragma unroll
+  for (uint32_t u = 0; u < kVectors; ++u) {
+    const uint32_t i = (u * kThreads + threadIdx.x) * 4, n = kWhole || i + 4 <= elems ? 4 : i < elems ? elems - i : 0;
+    g[u].template load<kStream>(grad + i, n);
+    p[u].template load<kStream>(param + i, n);
+    m[u].template load<kStream>(m_state + i, n);
+    v[u].template load<kStream>(v_state + i, n);
+    if constexpr (kEight) {
+      m_exponent[u] = n ? m_scale[i / kBlock] : 0;
+      v_exponent[u] = n ? v_scale[i / kBlock] : 0;
     }
-    if (!mine) continue;
-    const uint32_t scale_m = scale_of(top_m), scale_v = scale_of(top_v);
-    const uint32_t word = mix((uint32_t)i + (uint32_t)(i >> 32) * 0x632BE5ABu + key);
-    codes_m[i] = (uint8_t)code_of<false>(s.m, scale_m, word & 0xFFFFu);
-    codes_v[i] = (uint8_t)code_of<true>(s.root, scale_v, word >> 16);
-    if (i % kBlock == 0) {
-      scales_m[block] = (uint8_t)scale_m;
-      scales_v[block] = (uint8_t)scale_v;
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < kVectors; ++u) {
+    const uint32_t i = (u * kThreads + threadIdx.x) * 4, n = kWhole || i + 4 <= elems ? 4 : i < elems ? elems - i : 0;
+    float m_now[4], v_now[4], root[4];
+    uint32_t word[4];
+    if constexpr (kEight) {
+      values_of(__builtin_bit_cast(uint32_t, m[u].v), scale_value(m_exponent[u]) * launch.beta1, m_now);
+      values_of(__builtin_bit_cast(uint32_t, v[u].v), scale_value(v_exponent[u]), root);
     }
-    const float p = next_param(launch, to_float(*param), s);
-    if (sizeof(P) == 2 && launch.stochastic) {
-      uint32_t bits = __float_as_uint(p);
-      if (fabsf(p) < INFINITY) bits = (bits + (mix(word ^ 0x5BF03635u) & 0xFFFFu)) & 0xFFFF0000u;
-      *param = from_float<P>(__uint_as_float(bits));
-    } else {
-      *param = from_float<P>(p);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      const float gradient = to_float(g[u].v[e]) * factor;
+      const float beta_m = kEight ? m_now[e] : (float)m[u].v[e] * launch.beta1, v_old = kEight ? root[e] * root[e] : (float)v[u].v[e];
+      m_now[e] = beta_m + gradient * launch.one_minus_beta1;
+      v_now[e] = v_old * launch.beta2 + gradient * gradient * launch.one_minus_beta2;
+      if (kEight || stochastic) word[e] = word_of(first + i + e, key);
     }
-    if (it.copy) static_cast<C*>(it.copy)[i] = from_float<C>(p);
+    roots_of(v_now, root);
+    Four<C> c;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      const float q = next_param(launch, to_float(p[u].v[e]), m_now[e], root[e]);
+      p[u].v[e] = stored_param<P>(q, stochastic, word[e]);
+      c.v[e] = from_float<C>(q);
+      if constexpr (!kEight) {
+        m[u].v[e] = m_now[e];
+        v[u].v[e] = v_now[e];
+      }
+    }
+    if constexpr (kEight) {  // (lanes without elements hold zeros, and come along to their block's largest value)
+      m[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<false>(m_now, word, m_exponent[u]));
+      v[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<true>(root, word, v_exponent[u]));
+      if (n && threadIdx.x % (kBlock / 4) == 0) {
+        m_scale[i / kBlock] = (uint8_t)m_exponent[u];
+        v_scale[i / kBlock] = (uint8_t)v_exponent[u];
+      }
+    }
+    p[u].template store<kStream>(param + i, n);
+    m[u].template store<kStream>(m_state + i, n);
+    v[u].template store<kStream>(v_state + i, n);
+    if (copy) c.template store<false>(copy + i, n);
   }
 }
 
+template <class P, class G, class C, bool kEight, bool kStream>
+__global__ __launch_bounds__(adamw_shape(kEight).threads) __attribute__((amdgpu_waves_per_eu(1, adamw_shape(kEight).waves))) void adamw_kernel(
+    AdamwLaunch launch) {
+  constexpr uint32_t kTile = adamw_shape(kEight).tile();
+  const uint32_t k = item_of(launch, blockIdx.x);
+  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kTile, left = launch.items[k].elems - first;
+  if (left >= kTile) adamw_tile<P, G, C, kEight, kStream, true>(launch, k, first, kTile);
+  else adamw_tile<P, G, C, kEight, kStream, false>(launch, k, first, (uint32_t)left);
+}
+
+// Sixteen values to a lane, in four steps of a workgroup's 1024.
+constexpr uint32_t kDequantizeTile = 4 * 1024;
 template <class T>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, const uint8_t* scales, T* values, uint64_t elems) {
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (uint64_t)gridDim.x * 256)
-    values[i] = from_float<T>(value_of(codes[i], scales[i / kBlock]));
+  const uint64_t first = (uint64_t)blockIdx.x * kDequantizeTile + threadIdx.x * 4;
+  Four<uint8_t> four[4];
+  uint32_t scale[4], n[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint64_t i = first + u * 1024;
+    n[u] = i + 4 <= elems ? 4 : i < elems ? (uint32_t)(elems - i) : 0;
+    four[u].load<false>(codes + i, n[u]);
+    scale[u] = n[u] ? scales[i / kBlock] : 0;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    float x[4];
+    values_of(__builtin_bit_cast(uint32_t, four[u].v), scale_value(scale[u]), x);
+    Four<T> out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out.v[e] = from_float<T>(x[e]);
+    out.template store<false>(values + first + u * 1024, n[u]);
+  }
 }
 
 template <class Body>
@@ -186,9 +362,10 @@ int with_type(int32_t dtype, Body body) {
 
 }  // namespace
 
-int launch_squared_norm(int32_t dtype, const SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream) {
+int launch_squared_norm(int32_t dtype, bool stream_past_caches, const SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream) {
   return with_type(dtype, [&](auto t) {
-    squared_norm_kernel<decltype(t)><<<blocks, 256, 0, (hipStream_t)stream>>>(launch, partials);
+    if (stream_past_caches) squared_norm_kernel<decltype(t), true><<<blocks, 256, 0, (hipStream_t)stream>>>(launch, partials);
+    else squared_norm_kernel<decltype(t), false><<<blocks, 256, 0, (hipStream_t)stream>>>(launch, partials);
     return (int)hipGetLastError();
   });
 }
@@ -198,11 +375,18 @@ int launch_squared_norm_total(const double* partials, uint32_t n, float* result,
   return (int)hipGetLastError();
 }
 
-int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, const AdamwLaunch& launch, void* stream) {
+int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, bool stream_past_caches, const AdamwLaunch& launch, void* stream) {
   return with_type(grad, [&](auto g) {
     const auto with_param = [&](auto p, auto c) {
-      if (state_bits == 8) adamw8_kernel<decltype(p), decltype(g), decltype(c)><<<launch.n_tiles, kAdamwThreads, 0, (hipStream_t)stream>>>(launch);
-      else adamw_kernel<decltype(p), decltype(g), decltype(c)><<<launch.n_tiles, kAdamwThreads, 0, (hipStream_t)stream>>>(launch);
+      using P = decltype(p);
+      using G = decltype(g);
+      using C = decltype(c);
+      hipStream_t s = (hipStream_t)stream;
+      const uint32_t threads = adamw_shape(state_bits == 8).threads;
+      if (state_bits == 8 && stream_past_caches) adamw_kernel<P, G, C, true, true><<<launch.n_tiles, threads, 0, s>>>(launch);
+      else if (state_bits == 8) adamw_kernel<P, G, C, true, false><<<launch.n_tiles, threads, 0, s>>>(launch);
+      else if (stream_past_caches) adamw_kernel<P, G, C, false, true><<<launch.n_tiles, threads, 0, s>>>(launch);
+      else adamw_kernel<P, G, C, false, false><<<launch.n_tiles, threads, 0, s>>>(launch);
       return (int)hipGetLastError();
     };
     if (param == ODC_OPS_BF16) return with_param(bf16(), bf16());
@@ -212,8 +396,7 @@ int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, 
 
 int launch_dequantize(const void* codes, const void* scales, void* values, uint64_t elems, int32_t dtype, void* stream) {
   return with_type(dtype, [&](auto t) {
-    const uint64_t blocks = (elems + 255) / 256;
-    dequantize_kernel<decltype(t)><<<(uint32_t)(blocks < 65536 ? blocks : 65536), 256, 0, (hipStream_t)stream>>>(
+    dequantize_kernel<decltype(t)><<<(uint32_t)((elems + kDequantizeTile - 1) / kDequantizeTile), 256, 0, (hipStream_t)stream>>>(
         static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<decltype(t)*>(values), elems);
     return (int)hipGetLastError();
   });

@@ -11,21 +11,25 @@ using namespace odc_ops_launch;
 // rows in registers
 // ------------------------------------------------------------------------------------------------
 // kElems neighbouring elements of a row from element i on; what lies behind the row's end is zero, and neither read
-// nor written. kBuffer: rows start at multiples of 16 bytes and end with a whole piece, and all lanes agree on the
-// row. It is then a buffer of its own to the hardware, whose bounds check takes the place of branches around the
-// accesses (which had cost the backward pass 20 registers).
-template <int kElems, class T, bool kBuffer>
+// nor written. kAccess says how:
+// kPlainRows: at any alignment, the piece at the row's end element by element;
+// kBufferRows: rows start at multiples of 16 bytes and end with a whole piece, and all lanes agree on the row. It is a
+// buffer of its own to the hardware, whose bounds check takes the place of branches around the accesses (with them the
+// passes over 16384 x 14336 bf16 took 368 and 691 us instead of 333 and 379);
+// kStreamRows: the same, nontemporal.
+template <int kElems, class T, RowAccess kAccess>
 struct Piece {
   static constexpr int kVectors = kElems / Vector<T>::kElems;
+  static constexpr int kPolicy = kAccess == kStreamRows ? 2 : 0;  // of a buffer access: nontemporal
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   typename Vector<T>::type v[kVectors];
 
   __device__ __forceinline__ void load(const T* row, uint32_t i, uint32_t width) {
-    if constexpr (kBuffer) {
+    if constexpr (kAccess != kPlainRows) {
       const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, width * sizeof(T), 0x00027000);
 #pragma unroll
       for (int k = 0; k < kVectors; ++k)
-        v[k] = __builtin_bit_cast(typename Vector<T>::type, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(buffer, i * sizeof(T) + k * 16, 0, 0));
+        v[k] = __builtin_bit_cast(typename Vector<T>::type, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(buffer, i * sizeof(T) + k * 16, 0, kPolicy));
     } else if (i + kElems <= width) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) v[k] = *reinterpret_cast<const typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems);
@@ -35,11 +39,11 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void store(T* row, uint32_t i, uint32_t width) const {
-    if constexpr (kBuffer) {
+    if constexpr (kAccess != kPlainRows) {
       const auto buffer = __builtin_amdgcn_make_buffer_rsrc(row, 0, width * sizeof(T), 0x00027000);
 #pragma unroll
       for (int k = 0; k < kVectors; ++k)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), buffer, i * sizeof(T) + k * 16, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), buffer, i * sizeof(T) + k * 16, 0, kPolicy);
     } else if (i + kElems <= width) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) *reinterpret_cast<typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems) = v[k];
@@ -58,6 +62,9 @@ struct Piece {
     for (int k = 0; k < kVectors; ++k) asm("" : "+v"(reinterpret_cast<u32x4&>(v[k])));
   }
 };
+
+// The same access for what stays in the caches: weights, which every workgroup reads.
+constexpr RowAccess kept(RowAccess access) { return access == kStreamRows ? kBufferRows : access; }
 
 // Which of a workgroup's rows a thread works on: the same for all of a wavefront where a row takes one or more, which
 // keeps the rows' addresses in scalar registers.
@@ -87,14 +94,14 @@ __device__ __forceinline__ void row_sums(float (&x)[kValues], float* scratch) {
   }
 }
 
-template <class T, class W, int kLanes, int kVectors, bool kBuffer, bool kAdd>
+template <class T, class W, int kLanes, int kVectors, RowAccess kAccess, bool kAdd>
 __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads) void norm_forward_kernel(odc_norm_forward c) {
   constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
   constexpr int kElems = Vector<T>::kElems;
   __shared__ float scratch[2][kThreads / 64];
   const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes;
   const float per_element = 1.0f / (float)width;
-  Piece<kElems, W, kBuffer> weight[kVectors], bias[kVectors];
+  Piece<kElems, W, kept(kAccess)> weight[kVectors], bias[kVectors];
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     const uint32_t i = (k * kLanes + lane) * kElems;
@@ -113,12 +120,12 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
   }
   constexpr uint32_t kRows = kThreads / kLanes;  // at once
   uint64_t row = (uint64_t)blockIdx.x * kRows + row_slot<kLanes>();
-  Piece<kElems, T, kBuffer> x[kVectors], r[kVectors];
-  const auto load = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors], const void* rows, uint64_t stride) {
+  Piece<kElems, T, kAccess> x[kVectors], r[kVectors];
+  const auto load = [&](Piece<kElems, T, kAccess>(&piece)[kVectors], const void* rows, uint64_t stride) {
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows ? width : 0);
   };
-  const auto load_row = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors]) {
+  const auto load_row = [&](Piece<kElems, T, kAccess>(&piece)[kVectors]) {
     load(piece, c.input, c.input_stride);
     if constexpr (kAdd) load(r, c.residual, c.residual_stride);
   };
@@ -140,7 +147,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 #pragma unroll
       for (int e = 0; e < kElems; ++e) sum[0] += x[k][e];
     const uint64_t here = row;
-    Piece<kElems, T, kBuffer> next[kVectors];
+    Piece<kElems, T, kAccess> next[kVectors];
     row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
     if constexpr (kAhead) load_row(next);
     row_sums<kLanes>(sum, scratch[0]);
@@ -152,7 +159,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
     for (int k = 0; k < kVectors; ++k)
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
-        const float d = (k * kLanes + lane) * kElems + (kBuffer ? 0 : e) < width ? x[k][e] - mean : 0.0f;
+        const float d = (k * kLanes + lane) * kElems + (kAccess != kPlainRows ? 0 : e) < width ? x[k][e] - mean : 0.0f;
         squares[0] += d * d;
       }
     row_sums<kLanes>(squares, scratch[1]);
@@ -175,7 +182,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 // A workgroup passes over rows blockIdx.x, + gridDim.x, ... (kThreads / kLanes of them at once), writes their
 // grad_input and keeps the sums for weight and bias of its lanes' columns in registers; at the end the rows that it had
 // at once are added in LDS, upper half onto lower half, and go to its row of the workspace.
-template <class T, class W, int kLanes, int kVectors, bool kBuffer>
+template <class T, class W, int kLanes, int kVectors, RowAccess kAccess>
 __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_backward_kernel(odc_norm_backward c) {
   constexpr int kThreads = backward_threads({kLanes, kVectors}), kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
   constexpr int kSums = 2 * kVectors * kElems;  // of a thread
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
   // The weights of a lane's columns stay in registers, or, where the sums and the rows need these, in LDS: every lane
   // puts its own there.
   constexpr bool kWeightInLds = kVectors > 1;
-  typedef Piece<kElems, W, kBuffer> Weight;
+  typedef Piece<kElems, W, kept(kAccess)> Weight;
   __shared__ typename Vector<W>::type weights[kWeightInLds ? kVectors * Weight::kVectors * kThreads : 1];
   Weight weight_here[kWeightInLds ? 1 : kVectors];
   float dw[kVectors][kElems] = {}, db[kVectors][kElems] = {};
@@ -216,9 +223,9 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
   };
   int parity = 0;
   uint64_t row = (uint64_t)blockIdx.x * kRows + slot;
-  Piece<kElems, T, kBuffer> x[kVectors], dy[kVectors], dt[kVectors];
+  Piece<kElems, T, kAccess> x[kVectors], dy[kVectors], dt[kVectors];
   float mean, rstd;
-  const auto load = [&](Piece<kElems, T, kBuffer>(&piece)[kVectors], const void* rows, uint64_t stride) {
+  const auto load = [&](Piece<kElems, T, kAccess>(&piece)[kVectors], const void* rows, uint64_t stride) {
 #pragma unroll
     for (int k = 0; k < kVectors; ++k)
       piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows && rows ? width : 0);
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
     rstd = row < c.rows ? c.rstd[row] : 0;
   };
   // Where registers allow, the next row is on its way while this one's sums are made.
-  constexpr bool kAhead = kBuffer || kVectors == 1;
+  constexpr bool kAhead = kAccess != kPlainRows || kVectors == 1;
   if constexpr (kAhead) load_row();
   // every thread makes the same number of rounds: there are barriers in them
   for (uint64_t first = (uint64_t)blockIdx.x * kRows; first < c.rows; first += (uint64_t)gridDim.x * kRows, parity ^= 1) {
@@ -252,7 +259,7 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
     }
     const uint64_t here = row;
     const float mean_here = mean, rstd_here = rstd;
-    Piece<kElems, T, kBuffer> x_here[kVectors], dy_here[kVectors];
+    Piece<kElems, T, kAccess> x_here[kVectors], dy_here[kVectors];
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) x_here[k] = x[k], dy_here[k] = dy[k];
     if (c.grad_input) load(dt, c.grad_total, c.grad_total_stride);
@@ -473,11 +480,14 @@ void with_truth(bool truth, Body body) {
   else body(Number<0>());
 }
 
-// Rows that share a wavefront are no buffers (the plan does not ask for it).
+// Rows that share a wavefront are no buffers (access_of in odc_ops_host.cpp does not say so either).
 template <int kLanes, class Body>
-void with_buffers(bool buffers, Body body) {
-  if constexpr (kLanes >= 64) with_truth(buffers, body);
-  else body(Number<0>());
+void with_access(RowAccess access, Body body) {
+  if constexpr (kLanes >= 64) {
+    if (access == kStreamRows) return body(Number<kStreamRows>());
+    if (access == kBufferRows) return body(Number<kBufferRows>());
+  }
+  body(Number<kPlainRows>());
 }
 
 }  // namespace
@@ -493,9 +503,9 @@ int launch_norm_forward(const odc_norm_forward& call, const NormForwardPlan& pla
       with_shape<kForwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
         constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
         constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
-        with_buffers<kLanes>(plan.buffers, [&](auto buffers) {
+        with_access<kLanes>(plan.access, [&](auto access) {
           with_truth(call.residual != nullptr, [&](auto add) {
-            norm_forward_kernel<T, W, kLanes, kVectors, decltype(buffers)::value, decltype(add)::value><<<plan.blocks, kThreads, 0, s>>>(call);
+            norm_forward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value, decltype(add)::value><<<plan.blocks, kThreads, 0, s>>>(call);
           });
         });
       });
@@ -513,8 +523,8 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
     if (plan.shape.lanes && plan.groups) {
       with_shape<kBackwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
         constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
-        with_buffers<kLanes>(plan.buffers, [&](auto buffers) {
-          norm_backward_kernel<T, W, kLanes, kVectors, decltype(buffers)::value><<<plan.groups, backward_threads(plan.shape), 0, s>>>(call);
+        with_access<kLanes>(plan.access, [&](auto access) {
+          norm_backward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value><<<plan.groups, backward_threads(plan.shape), 0, s>>>(call);
         });
       });
     } else if (plan.groups) {

@@ -36,6 +36,8 @@ bool spans_too_much(uint64_t rows, uint64_t stride, uint64_t width) {
   return width > kMost || rows > kMost || (rows && stride > kMost / rows);
 }
 
+constexpr uint64_t kLastLevelCache = uint64_t(256) << 20;
+
 // ---- layer norm -----------------------------------------------------------------------------------
 int check_norm(uint64_t rows, uint64_t width, int32_t dtype, int32_t weight_dtype) {
   if (!is_float_type(dtype) || !is_float_type(weight_dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d or %d", dtype, weight_dtype);
@@ -61,19 +63,30 @@ int check_rows(const char* name, const void* p, uint64_t rows, uint64_t width, u
 
 constexpr uint64_t kCus = 256;
 
-// Whether rows of whole 16 byte vectors start at multiples of 16 bytes. (A wavefront has one row or a part of one then:
-// kLanes is 64 at least.)
+// Whether rows of whole 16 byte vectors start at multiples of 16 bytes.
 bool rows_of_vectors(const void* p, uint64_t stride, int32_t dtype) { return aligned(p, 16) && stride * bytes_of(dtype) % 16 == 0; }
 
-bool buffers(const odc_norm_forward& c, const NormShape& shape) {
-  return shape.lanes >= 64 && rows_of_vectors(c.input, c.input_stride, c.dtype) && rows_of_vectors(c.residual, c.residual_stride, c.dtype) &&
-         rows_of_vectors(c.output, c.width, c.dtype) && rows_of_vectors(c.total, c.width, c.dtype) && aligned(c.weight, 16) && aligned(c.bias, 16);
+// What a pass reads and writes beyond the last-level cache's 256 MB is streamed past the caches: nothing of it would be
+// found again. us, in the caches / streamed: 16384 x 14336 bf16 with a residual (1.9 GB a pass) forward 336 / 326,
+// backward 380 / 330; 4096 x 4096 (134 MB) 24.7 / 30.0 and 31.8 / 33.7.
+// (A wavefront has one row or a part of one: lanes is 64 at least.)
+RowAccess access_of(bool vectors, const NormShape& shape, uint64_t rows, uint64_t width, int32_t dtype, int tensors) {
+  if (!vectors || shape.lanes < 64) return kPlainRows;
+  return rows * width * bytes_of(dtype) > kLastLevelCache / tensors ? kStreamRows : kBufferRows;
 }
 
-bool buffers(const odc_norm_backward& c, const NormShape& shape) {
-  return shape.lanes >= 64 && rows_of_vectors(c.grad_output, c.grad_output_stride, c.dtype) &&
-         rows_of_vectors(c.grad_total, c.grad_total_stride, c.dtype) && rows_of_vectors(c.normalised, c.normalised_stride, c.dtype) &&
-         c.width * bytes_of(c.dtype) % 16 == 0 && aligned(c.grad_input, 16) && aligned(c.weight, 16);
+RowAccess access_of(const odc_norm_forward& c, const NormShape& shape) {
+  const bool vectors = rows_of_vectors(c.input, c.input_stride, c.dtype) && rows_of_vectors(c.residual, c.residual_stride, c.dtype) &&
+                       rows_of_vectors(c.output, c.width, c.dtype) && rows_of_vectors(c.total, c.width, c.dtype) && aligned(c.weight, 16) &&
+                       aligned(c.bias, 16);
+  return access_of(vectors, shape, c.rows, c.width, c.dtype, c.residual ? 4 : 2);
+}
+
+RowAccess access_of(const odc_norm_backward& c, const NormShape& shape) {
+  const bool vectors = rows_of_vectors(c.grad_output, c.grad_output_stride, c.dtype) && rows_of_vectors(c.grad_total, c.grad_total_stride, c.dtype) &&
+                       rows_of_vectors(c.normalised, c.normalised_stride, c.dtype) && rows_of_vectors(c.grad_input, c.width, c.dtype) &&
+                       aligned(c.weight, 16);
+  return access_of(vectors, shape, c.rows, c.width, c.dtype, 2 + (c.grad_total != nullptr) + (c.grad_input != nullptr));
 }
 
 NormForwardPlan forward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
@@ -124,6 +137,13 @@ int check_elems(uint64_t elems, uint32_t i, uint32_t tile) {
   return ODC_OPS_OK;
 }
 
+template <class Item>
+uint64_t all_elems(const Item* items, uint32_t n_items) {
+  uint64_t sum = 0;
+  for (uint32_t i = 0; i < n_items; ++i) sum += items[i].elems;
+  return sum;
+}
+
 uint32_t partials_of(uint32_t n_tiles) { return std::min(n_tiles, kMostPartials); }
 
 }  // namespace
@@ -147,7 +167,7 @@ int odc_layer_norm(const odc_norm_forward* call, void* stream) {
   ODC_OPS_TRY(check_rows("bias", c.bias, 1, c.width, c.width, c.weight_dtype, false));
   if (!aligned(c.mean, 4) || !aligned(c.rstd, 4)) return fail(ODC_OPS_ERR_INVALID, "mean or rstd is not aligned to its element");
   NormForwardPlan plan = forward_plan(c.rows, c.width, c.dtype);
-  plan.buffers = buffers(c, plan.shape);
+  plan.access = access_of(c, plan.shape);
   return launched(odc_ops_device::launch_norm_forward(c, plan, stream));
 }
 
@@ -177,7 +197,7 @@ int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {
     if (!aligned(c.workspace, 16)) return fail(ODC_OPS_ERR_INVALID, "the workspace is not aligned to 16 bytes");
   }
   NormBackwardPlan plan = backward_plan(c.rows, c.width, c.dtype);
-  plan.buffers = buffers(c, plan.shape);
+  plan.access = access_of(c, plan.shape);
   return launched(odc_ops_device::launch_norm_backward(c, plan, stream));
 }
 
@@ -207,6 +227,7 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
     return fail(ODC_OPS_ERR_INVALID, "the workspace needs %llu bytes, aligned to 8", (unsigned long long)need);
   if (need / sizeof(double) > 0xffffffffu) return fail(ODC_OPS_ERR_INVALID, "too many items");
+  const bool past_caches = all_elems(items, n_items) > kLastLevelCache / bytes_of(dtype);
   double* partials = static_cast<double*>(workspace);
   uint32_t done = 0;
   SquaredNormLaunch launch;
@@ -214,7 +235,7 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
     at = fill_table(launch, items, n_items, at, kNormItems, kNormTile);
     const uint32_t blocks = partials_of(launch.n_tiles);
     if (!blocks) continue;
-    ODC_OPS_TRY(launched(odc_ops_device::launch_squared_norm(dtype, launch, blocks, partials + done, stream)));
+    ODC_OPS_TRY(launched(odc_ops_device::launch_squared_norm(dtype, past_caches, launch, blocks, partials + done, stream)));
     done += blocks;
   }
   return launched(odc_ops_device::launch_squared_norm_total(partials, done, result, stream));
@@ -236,10 +257,11 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
   if (!(a.grad_scale >= 0) || !std::isfinite(a.grad_scale)) return fail(ODC_OPS_ERR_INVALID, "grad_scale is finite and not negative");
   if (a.squared_norm && (!(a.max_norm >= 0) || !aligned(a.squared_norm, 4)))
     return fail(ODC_OPS_ERR_INVALID, "max_norm is not negative, squared_norm aligned to its element");
+  const uint32_t tile = adamw_shape(a.state_bits == 8).tile();
   for (uint32_t i = 0; i < n_items; ++i) {
     const odc_adamw_item& it = items[i];
     if (!it.elems) continue;
-    ODC_OPS_TRY(check_elems(it.elems, i, kAdamwTile));
+    ODC_OPS_TRY(check_elems(it.elems, i, tile));
     if (!it.param || !it.grad || !it.exp_avg || !it.exp_avg_sq) return fail(ODC_OPS_ERR_INVALID, "item %u: a pointer is NULL", i);
     if (a.state_bits == 8 && (!it.exp_avg_scale || !it.exp_avg_sq_scale)) return fail(ODC_OPS_ERR_INVALID, "item %u: scales are NULL", i);
     if ((a.copy_dtype != ODC_OPS_NONE) != (it.copy != nullptr)) return fail(ODC_OPS_ERR_INVALID, "item %u: copies of all tensors or of none", i);
@@ -247,6 +269,8 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
         (a.state_bits == 32 && (!aligned(it.exp_avg, 4) || !aligned(it.exp_avg_sq, 4))))
       return fail(ODC_OPS_ERR_INVALID, "item %u: a pointer is not aligned to its element", i);
   }
+  const uint32_t bytes = 2 * bytes_of(a.param_dtype) + bytes_of(a.grad_dtype) + (a.state_bits == 32 ? 16 : 4);
+  const bool past_caches = all_elems(items, n_items) > kLastLevelCache / bytes;
   const double t = (double)a.step;
   AdamwLaunch launch;
   launch.beta1 = (float)a.beta1;
@@ -264,9 +288,9 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
   launch.stochastic = a.stochastic != 0;
   for (uint32_t at = 0; at < n_items;) {
     launch.first_item = at;
-    at = fill_table(launch, items, n_items, at, kAdamwItems, kAdamwTile);
+    at = fill_table(launch, items, n_items, at, kAdamwItems, tile);
     if (!launch.n_tiles) continue;
-    ODC_OPS_TRY(launched(odc_ops_device::launch_adamw(a.param_dtype, a.grad_dtype, a.copy_dtype, a.state_bits, launch, stream)));
+    ODC_OPS_TRY(launched(odc_ops_device::launch_adamw(a.param_dtype, a.grad_dtype, a.copy_dtype, a.state_bits, past_caches, launch, stream)));
   }
   return ODC_OPS_OK;
 }
@@ -275,7 +299,7 @@ int odc_dequantize_blocks(const void* codes, const void* scales, void* values, u
   if (!is_float_type(dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
   if (!elems) return ODC_OPS_OK;
   if (!codes || !scales || !values || !aligned(values, bytes_of(dtype))) return fail(ODC_OPS_ERR_INVALID, "a pointer is NULL or not aligned");
-  if (elems > uint64_t(1) << 40) return fail(ODC_OPS_ERR_INVALID, "%llu elements are too many", (unsigned long long)elems);
+  if (ceil_div(elems, 1024) > kMostTiles) return fail(ODC_OPS_ERR_INVALID, "%llu elements are too many", (unsigned long long)elems);
   return launched(odc_ops_device::launch_dequantize(codes, scales, values, elems, dtype, stream));
 }
 

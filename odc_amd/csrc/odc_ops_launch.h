@@ -36,9 +36,12 @@ inline NormShape shape_of(const NormShape (&shapes)[n], uint64_t width, int32_t 
   return {0, 0};
 }
 
+// How rows in registers are read and written (Piece in odc_norm_kernels.hip, access_of in odc_ops_host.cpp).
+enum RowAccess : uint32_t { kPlainRows, kBufferRows, kStreamRows };
+
 struct NormForwardPlan {
   NormShape shape;
-  bool buffers;  // every row is a buffer of whole vectors (Piece in odc_norm_kernels.hip)
+  RowAccess access;
   uint32_t blocks;
 };
 
@@ -46,7 +49,7 @@ struct NormForwardPlan {
 // into its row of the workspace ([groups][2][width] floats), and a second launch adds the groups.
 struct NormBackwardPlan {
   NormShape shape;
-  bool buffers;
+  RowAccess access;
   uint32_t groups;
   uint32_t row_blocks;      // wide rows: workgroups of the pass over rows
   uint64_t rows_per_group;  // wide rows: of the pass over columns
@@ -55,7 +58,7 @@ constexpr uint32_t kColumnTile = 64;  // columns of one workgroup of the passes 
 
 // ---- lists of tensors -----------------------------------------------------------------------------
 // A dispatch counts its work-items in 32 bits: the most workgroups of 256.
-constexpr uint32_t kMostTiles = 0xffffffffu / 256;
+constexpr uint32_t kMostTiles = 0xffffffffu / 256;  // (a launch of fewer threads could have more)
 // A launch has a table of its tensors and the number of the first tile of each.
 constexpr uint32_t kNormItems = 160;
 constexpr uint32_t kNormTile = 8192;  // elements of a tile of the squared norm
@@ -69,8 +72,19 @@ static_assert(sizeof(SquaredNormLaunch) <= 3800, "kernel arguments are limited t
 
 constexpr uint32_t kBlock = 32;  // elements of a state in 8 bits that share a scale
 constexpr uint32_t kAdamwItems = 48;
-constexpr uint32_t kAdamwTile = 1024;  // elements
-constexpr uint32_t kAdamwThreads = 256;
+// A workgroup of the AdamW step: its threads, how many vectors of four elements a lane has, and how many wavefronts a SIMD
+// may hold (a bound in the kernel's own attributes).
+struct AdamwShape {
+  uint32_t threads, vectors, waves;
+  constexpr uint32_t tile() const { return threads * vectors * 4; }
+};
+#ifndef S8
+#define S8 256, 2, 8
+#endif
+#ifndef S32
+#define S32 64, 1, 3
+#endif
+constexpr AdamwShape adamw_shape(bool eight) { return eight ? AdamwShape{S8} : AdamwShape{S32}; }
 struct AdamwLaunch {
   float beta1, beta2, one_minus_beta1, one_minus_beta2;
   float decay;          // 1 - lr * weight_decay
@@ -92,9 +106,10 @@ namespace odc_ops_device {
 // Each returns 0 or a hipError_t.
 int launch_norm_forward(const odc_norm_forward& call, const odc_ops_launch::NormForwardPlan& plan, void* stream);
 int launch_norm_backward(const odc_norm_backward& call, const odc_ops_launch::NormBackwardPlan& plan, void* stream);
-int launch_squared_norm(int32_t dtype, const odc_ops_launch::SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream);
+int launch_squared_norm(int32_t dtype, bool stream_past_caches, const odc_ops_launch::SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream);
 int launch_squared_norm_total(const double* partials, uint32_t n, float* result, void* stream);
-int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, const odc_ops_launch::AdamwLaunch& launch, void* stream);
+int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, bool stream_past_caches, const odc_ops_launch::AdamwLaunch& launch,
+                 void* stream);
 int launch_dequantize(const void* codes, const void* scales, void* values, uint64_t elems, int32_t dtype, void* stream);
 const char* error_string(int code);
 

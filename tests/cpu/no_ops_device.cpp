@@ -26,7 +26,7 @@ int answer = 0;
 namespace odc_ops_device {
 int launch_norm_forward(const odc_norm_forward&, const NormForwardPlan&, void*) { return ++seen.norm_forward, answer; }
 int launch_norm_backward(const odc_norm_backward&, const NormBackwardPlan&, void*) { return ++seen.norm_backward, answer; }
-int launch_squared_norm(int32_t, const SquaredNormLaunch& launch, uint32_t blocks, double* partials, void*) {
+int launch_squared_norm(int32_t, bool, const SquaredNormLaunch& launch, uint32_t blocks, double* partials, void*) {
   seen.squared.push_back(launch);
   seen.squared_blocks.push_back(blocks);
   seen.squared_partials.push_back(partials);
@@ -37,7 +37,7 @@ int launch_squared_norm_total(const double*, uint32_t n, float*, void*) {
   seen.total_partials = n;
   return answer;
 }
-int launch_adamw(int32_t, int32_t, int32_t, int32_t, const AdamwLaunch& launch, void*) { return seen.adamw.push_back(launch), answer; }
+int launch_adamw(int32_t, int32_t, int32_t, int32_t, bool, const AdamwLaunch& launch, void*) { return seen.adamw.push_back(launch), answer; }
 int launch_dequantize(const void*, const void*, void*, uint64_t, int32_t, void*) { return ++seen.dequantize, answer; }
 const char* error_string(int) { return "no device"; }
 }  // namespace odc_ops_device
@@ -161,7 +161,7 @@ void check_lists() {
       seen = Seen();
       odc_adamw_numbers a = {1e-3, 0.9, 0.999, 1e-8, 0.1, 1.0, 0.0, nullptr, 3, 7, 0, ODC_OPS_F32, ODC_OPS_BF16, ODC_OPS_NONE, bits};
       CHECK(odc_adamw(items.data(), (uint32_t)items.size(), &a, nullptr) == ODC_OPS_OK);
-      check_tables(seen.adamw, items, kAdamwTile);
+      check_tables(seen.adamw, items, adamw_shape(bits == 8).tile());
       uint32_t first = 0;
       for (const AdamwLaunch& launch : seen.adamw) {
         while (first < launch.first_item) CHECK(items[first++].elems == 0);
