@@ -84,15 +84,19 @@ __device__ __forceinline__ T block_sum(T x, T* scratch) {
   return x;
 }
 
-// The item of a tile: the last one whose first tile is not behind it (items without elements have no tile).
+// The item of a tile: the last one whose first tile is not behind it (items without elements have no tile). Each lane
+// looks at an item of its own, where a binary search would wait for the table several times over.
 template <class Launch>
 __device__ __forceinline__ uint32_t item_of(const Launch& launch, uint32_t tile) {
-  uint32_t low = 0, high = launch.n_items;
-  while (high - low > 1) {
-    const uint32_t mid = (low + high) / 2;
-    if (launch.first_tile[mid] <= tile) low = mid; else high = mid;
+  constexpr uint32_t kItems = sizeof(launch.first_tile) / sizeof(uint32_t) - 1;
+  const uint32_t lane = threadIdx.x % 64;
+  uint32_t begun = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kItems; i += 64) {
+    const uint32_t k = i + lane;
+    begun += __popcll(__ballot(k < launch.n_items && launch.first_tile[k < kItems ? k : 0] <= tile));
   }
-  return low;
+  return __builtin_amdgcn_readfirstlane(begun) - 1;
 }
 
 }  // namespace odc_ops_device

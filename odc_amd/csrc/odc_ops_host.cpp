@@ -119,21 +119,21 @@ NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
 // ---- lists ----------------------------------------------------------------------------------------
 // Fills a launch's table with items from `at` on; returns the first item that is not in it.
 template <class Launch, class Item>
-uint32_t fill_table(Launch& launch, const Item* items, uint32_t n_items, uint32_t at, uint32_t most_items, uint32_t tile) {
+uint32_t fill_table(Launch& launch, const Item* items, uint32_t n_items, uint32_t at, uint32_t most_items, uint32_t tile, uint32_t threads) {
   launch.n_items = launch.n_tiles = 0;
   while (at < n_items && launch.n_items < most_items) {
     const uint64_t tiles = ceil_div(items[at].elems, tile);
-    if (tiles > kMostTiles - launch.n_tiles) break;  // (one tensor alone always fits: check_list)
+    if (tiles > most_workgroups(threads) - launch.n_tiles) break;  // (one tensor alone always fits: check_list)
     launch.first_tile[launch.n_items] = launch.n_tiles;
-    launch.items[launch.n_items++] = items[at++];
+    launch.set(launch.n_items++, items[at++]);
     launch.n_tiles += (uint32_t)tiles;
   }
   launch.first_tile[launch.n_items] = launch.n_tiles;
   return at;
 }
 
-int check_elems(uint64_t elems, uint32_t i, uint32_t tile) {
-  if (ceil_div(elems, tile) > kMostTiles) return fail(ODC_OPS_ERR_INVALID, "item %u: %llu elements are too many", i, (unsigned long long)elems);
+int check_elems(uint64_t elems, uint32_t i, uint32_t tile, uint32_t threads) {
+  if (ceil_div(elems, tile) > most_workgroups(threads)) return fail(ODC_OPS_ERR_INVALID, "item %u: %llu elements are too many", i, (unsigned long long)elems);
   return ODC_OPS_OK;
 }
 
@@ -206,8 +206,8 @@ uint64_t odc_squared_norm_workspace(const odc_span_item* items, uint32_t n_items
   uint64_t partials = 0;
   SquaredNormLaunch launch;
   for (uint32_t at = 0; at < n_items;) {
-    if (check_elems(items[at].elems, at, kNormTile) != ODC_OPS_OK) return 0;
-    at = fill_table(launch, items, n_items, at, kNormItems, kNormTile);
+    if (check_elems(items[at].elems, at, kNormTile, kNormThreads) != ODC_OPS_OK) return 0;
+    at = fill_table(launch, items, n_items, at, kNormItems, kNormTile, kNormThreads);
     partials += partials_of(launch.n_tiles);
   }
   return partials * sizeof(double);
@@ -219,8 +219,8 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
   if (!items && n_items) return fail(ODC_OPS_ERR_INVALID, "items is NULL");
   if (!is_float_type(dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
   for (uint32_t i = 0; i < n_items; ++i) {
-    ODC_OPS_TRY(check_elems(items[i].elems, i, kNormTile));
-    if (items[i].elems && (!items[i].data || !aligned(items[i].data, bytes_of(dtype))))
+    ODC_OPS_TRY(check_elems(items[i].elems, i, kNormTile, kNormThreads));
+    if (items[i].elems && (!items[i].data || !aligned(items[i].data, bytes_of(dtype)) || (uint64_t)(uintptr_t)items[i].data >> 48))
       return fail(ODC_OPS_ERR_INVALID, "item %u: data is NULL or not aligned to its element", i);
   }
   const uint64_t need = n_items ? odc_squared_norm_workspace(items, n_items, dtype) : 0;
@@ -232,7 +232,7 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
   uint32_t done = 0;
   SquaredNormLaunch launch;
   for (uint32_t at = 0; at < n_items;) {
-    at = fill_table(launch, items, n_items, at, kNormItems, kNormTile);
+    at = fill_table(launch, items, n_items, at, kNormItems, kNormTile, kNormThreads);
     const uint32_t blocks = partials_of(launch.n_tiles);
     if (!blocks) continue;
     ODC_OPS_TRY(launched(odc_ops_device::launch_squared_norm(dtype, past_caches, launch, blocks, partials + done, stream)));
@@ -257,11 +257,11 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
   if (!(a.grad_scale >= 0) || !std::isfinite(a.grad_scale)) return fail(ODC_OPS_ERR_INVALID, "grad_scale is finite and not negative");
   if (a.squared_norm && (!(a.max_norm >= 0) || !aligned(a.squared_norm, 4)))
     return fail(ODC_OPS_ERR_INVALID, "max_norm is not negative, squared_norm aligned to its element");
-  const uint32_t tile = adamw_shape(a.state_bits == 8).tile();
+  const AdamwShape shape = adamw_shape(a.state_bits == 8);
   for (uint32_t i = 0; i < n_items; ++i) {
     const odc_adamw_item& it = items[i];
     if (!it.elems) continue;
-    ODC_OPS_TRY(check_elems(it.elems, i, tile));
+    ODC_OPS_TRY(check_elems(it.elems, i, shape.tile(), shape.threads));
     if (!it.param || !it.grad || !it.exp_avg || !it.exp_avg_sq) return fail(ODC_OPS_ERR_INVALID, "item %u: a pointer is NULL", i);
     if (a.state_bits == 8 && (!it.exp_avg_scale || !it.exp_avg_sq_scale)) return fail(ODC_OPS_ERR_INVALID, "item %u: scales are NULL", i);
     if ((a.copy_dtype != ODC_OPS_NONE) != (it.copy != nullptr)) return fail(ODC_OPS_ERR_INVALID, "item %u: copies of all tensors or of none", i);
@@ -288,7 +288,7 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
   launch.stochastic = a.stochastic != 0;
   for (uint32_t at = 0; at < n_items;) {
     launch.first_item = at;
-    at = fill_table(launch, items, n_items, at, kAdamwItems, tile);
+    at = fill_table(launch, items, n_items, at, kAdamwItems, shape.tile(), shape.threads);
     if (!launch.n_tiles) continue;
     ODC_OPS_TRY(launched(odc_ops_device::launch_adamw(a.param_dtype, a.grad_dtype, a.copy_dtype, a.state_bits, past_caches, launch, stream)));
   }
@@ -299,7 +299,7 @@ int odc_dequantize_blocks(const void* codes, const void* scales, void* values, u
   if (!is_float_type(dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
   if (!elems) return ODC_OPS_OK;
   if (!codes || !scales || !values || !aligned(values, bytes_of(dtype))) return fail(ODC_OPS_ERR_INVALID, "a pointer is NULL or not aligned");
-  if (ceil_div(elems, 1024) > kMostTiles) return fail(ODC_OPS_ERR_INVALID, "%llu elements are too many", (unsigned long long)elems);
+  if (ceil_div(elems, 1024) > most_workgroups(256)) return fail(ODC_OPS_ERR_INVALID, "%llu elements are too many", (unsigned long long)elems);
   return launched(odc_ops_device::launch_dequantize(codes, scales, values, elems, dtype, stream));
 }
 

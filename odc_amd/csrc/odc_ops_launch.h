@@ -57,18 +57,26 @@ struct NormBackwardPlan {
 constexpr uint32_t kColumnTile = 64;  // columns of one workgroup of the passes over columns
 
 // ---- lists of tensors -----------------------------------------------------------------------------
-// A dispatch counts its work-items in 32 bits: the most workgroups of 256.
-constexpr uint32_t kMostTiles = 0xffffffffu / 256;  // (a launch of fewer threads could have more)
+// A dispatch counts its work-items in 32 bits.
+constexpr uint32_t most_workgroups(uint32_t threads) { return 0xffffffffu / threads; }
+
 // A launch has a table of its tensors and the number of the first tile of each.
-constexpr uint32_t kNormItems = 160;
+constexpr uint32_t kNormItems = 320;
+constexpr uint32_t kNormThreads = 256;
 constexpr uint32_t kNormTile = 8192;  // elements of a tile of the squared norm
 constexpr uint32_t kMostPartials = 2048;
 struct SquaredNormLaunch {
   uint32_t n_items, n_tiles;
   uint32_t first_tile[kNormItems + 1];
-  odc_span_item items[kNormItems];
+  // An item in 8 bytes, for a table of 320: its address (of 48 bits), and below it the elements of its last tile.
+  uint64_t places[kNormItems];
+
+  void set(uint32_t k, const odc_span_item& item) {
+    const uint64_t last = item.elems ? (item.elems - 1) % kNormTile + 1 : 0;
+    places[k] = (uint64_t)(uintptr_t)item.data << 16 | last;
+  }
 };
-static_assert(sizeof(SquaredNormLaunch) <= 3800, "kernel arguments are limited to 4 KiB");
+static_assert(sizeof(SquaredNormLaunch) <= 3900, "kernel arguments are limited to 4 KiB");
 
 constexpr uint32_t kBlock = 32;  // elements of a state in 8 bits that share a scale
 constexpr uint32_t kAdamwItems = 48;
@@ -96,6 +104,8 @@ struct AdamwLaunch {
   uint32_t n_items, n_tiles;
   uint32_t first_tile[kAdamwItems + 1];
   odc_adamw_item items[kAdamwItems];
+
+  void set(uint32_t k, const odc_adamw_item& item) { items[k] = item; }
 };
 static_assert(sizeof(AdamwLaunch) <= 3800, "kernel arguments are limited to 4 KiB");
 

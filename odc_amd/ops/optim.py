@@ -35,7 +35,7 @@ BLOCK = 32  # elements of a state in 8 bits that share a scale
 
 def squared_norm(tensors: Sequence[Tensor]) -> Tensor:
     """The sum of the squares of all elements of all tensors, as an fp32 scalar on their device: two launches for up
-    to 160 tensors, no round trip to the host. Shards of one model: sum it over the ranks (``all_reduce``) before
+    to 320 tensors, no round trip to the host. Shards of one model: sum it over the ranks (``all_reduce``) before
     clipping by it."""
     if not isinstance(tensors, (list, tuple)):
         tensors = list(tensors)

@@ -55,6 +55,12 @@ namespace {
 // Made-up device addresses: nothing here reads through them.
 void* at(uintptr_t address) { return reinterpret_cast<void*>(address); }
 
+void check_item(const AdamwLaunch& launch, uint32_t i, const odc_adamw_item& item) { CHECK(launch.items[i].elems == item.elems); }
+void check_item(const SquaredNormLaunch& launch, uint32_t i, const odc_span_item& item) {
+  const uint64_t tiles = launch.first_tile[i + 1] - launch.first_tile[i], last = launch.places[i] & 0xFFFF;
+  CHECK(launch.places[i] >> 16 == (uint64_t)(uintptr_t)item.data && (tiles ? (tiles - 1) * kNormTile + last : 0) == item.elems);
+}
+
 // The tables of a list's launches: every item in order, with as many tiles as its elements need.
 template <class Launch, class Item>
 void check_tables(const std::vector<Launch>& launches, const std::vector<Item>& items, uint32_t tile) {
@@ -62,7 +68,7 @@ void check_tables(const std::vector<Launch>& launches, const std::vector<Item>& 
   for (const Launch& launch : launches) {
     CHECK(launch.n_tiles > 0 && launch.first_tile[0] == 0 && launch.first_tile[launch.n_items] == launch.n_tiles);
     for (uint32_t i = 0; i < launch.n_items; ++i, ++k) {
-      CHECK(launch.items[i].elems == items[k].elems);
+      check_item(launch, i, items[k]);
       CHECK(launch.first_tile[i + 1] - launch.first_tile[i] == (items[k].elems + tile - 1) / tile);
     }
   }
@@ -216,7 +222,8 @@ void check_adamw_refusals() {
   CHECK(odc_dequantize_blocks(at(1), at(2), at(4), 10, 7, nullptr) < 0);
   CHECK(odc_dequantize_blocks(nullptr, nullptr, nullptr, 0, ODC_OPS_F32, nullptr) == ODC_OPS_OK && seen.dequantize == 1);
   float result;
-  const odc_span_item span = {at(0x1001), 10};
+  const odc_span_item span = {at(0x1001), 10}, far = {at(uintptr_t(1) << 48), 10};
+  CHECK(odc_squared_norm(&far, 1, ODC_OPS_F32, at(0x1000), 1 << 20, &result, nullptr) < 0);
   CHECK(odc_squared_norm(&span, 1, ODC_OPS_F32, at(0x1000), 1 << 20, &result, nullptr) < 0);
   CHECK(odc_squared_norm(&span, 1, 9, at(0x1000), 1 << 20, &result, nullptr) < 0);
   CHECK(odc_squared_norm(&span, 1, ODC_OPS_F32, at(0x1000), 1 << 20, nullptr, nullptr) < 0);
