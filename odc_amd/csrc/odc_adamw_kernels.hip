@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void squared_norm_kernel(SquaredNormLaunch lau
   __shared__ double scratch[4];
   double total = 0;
   for (uint32_t tile = blockIdx.x; tile < launch.n_tiles; tile += gridDim.x) {
-    const uint32_t k = item_of(launch, tile);
+    const uint32_t k = item_of_many(launch, tile);
     const uint64_t place = launch.places[k];
     const uint32_t tile_of_item = tile - launch.first_tile[k];
     const uint32_t left = tile + 1 < launch.first_tile[k + 1] ? kNormTile : (uint32_t)(place & 0xFFFF);

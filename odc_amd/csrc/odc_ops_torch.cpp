@@ -224,7 +224,7 @@ struct NormShape {
 };
 
 struct NormOutputs {
-  at::Tensor output, total, mean, rstd;
+  at::Tensor output, total, statistics;  // [2][rows]: means, and the reciprocals of the standard deviations
 };
 
 void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -240,8 +240,7 @@ NormOutputs norm_forward(const at::Tensor& input, const at::Tensor& residual, co
   out.output = at::empty(input.sizes(), input.options());
   if (residual.defined()) out.total = at::empty(input.sizes(), input.options());
   if (keep_statistics) {
-    out.mean = at::empty({shape.rows}, input.options().dtype(at::kFloat));
-    out.rstd = at::empty({shape.rows}, input.options().dtype(at::kFloat));
+    out.statistics = at::empty({2, shape.rows}, input.options().dtype(at::kFloat));
   }
   odc_norm_forward call = {};
   call.input = x.data();
@@ -250,8 +249,8 @@ NormOutputs norm_forward(const at::Tensor& input, const at::Tensor& residual, co
   call.bias = pointer(b);
   call.output = out.output.data_ptr();
   call.total = pointer(out.total);
-  call.mean = static_cast<float*>(pointer(out.mean));
-  call.rstd = static_cast<float*>(pointer(out.rstd));
+  call.mean = static_cast<float*>(pointer(out.statistics));
+  call.rstd = call.mean ? call.mean + shape.rows : nullptr;
   call.rows = (uint64_t)shape.rows;
   call.width = (uint64_t)shape.width;
   call.input_stride = x.stride;
@@ -279,7 +278,7 @@ struct Wanted {
 };
 
 NormGradients norm_backward(const at::Tensor& dy, const at::Tensor& dtotal, const at::Tensor& normalised, const at::Tensor& weight,
-                            const at::Tensor& mean, const at::Tensor& rstd, const NormShape& shape, at::ScalarType weight_type, Wanted wanted) {
+                            const at::Tensor& statistics, const NormShape& shape, at::ScalarType weight_type, Wanted wanted) {
   const c10::DeviceGuard guard(normalised.device());
   const Rows g(dy, shape.dims, shape.width), x(normalised, shape.dims, shape.width), t(dtotal, shape.dims, shape.width);
   const at::Tensor w = contiguous(weight);
@@ -297,8 +296,8 @@ NormGradients norm_backward(const at::Tensor& dy, const at::Tensor& dtotal, cons
   call.normalised = x.data();
   call.normalised_stride = x.stride;
   call.weight = pointer(w);
-  call.mean = static_cast<const float*>(mean.data_ptr());
-  call.rstd = static_cast<const float*>(rstd.data_ptr());
+  call.mean = static_cast<const float*>(statistics.data_ptr());
+  call.rstd = call.mean + shape.rows;
   const auto row_shape = normalised.sizes().slice((size_t)(normalised.dim() - shape.dims));
   if (wanted.input) {
     out.input = at::empty(normalised.sizes(), normalised.options());
@@ -328,9 +327,9 @@ NormGradients norm_backward(const at::Tensor& dy, const at::Tensor& dtotal, cons
 class LayerNormBackward : public torch::autograd::Function<LayerNormBackward> {
  public:
   static variable_list forward(AutogradContext*, const at::Tensor& dy, const Optional& dtotal, const at::Tensor& normalised, const Optional& weight,
-                               const at::Tensor& mean, const at::Tensor& rstd, const NormShape& shape, at::ScalarType weight_type, Wanted wanted) {
-    const NormGradients out = norm_backward(dy, dtotal.value_or(at::Tensor()), normalised, weight.value_or(at::Tensor()), mean, rstd, shape,
-                                            weight_type, wanted);
+                               const at::Tensor& statistics, const NormShape& shape, at::ScalarType weight_type, Wanted wanted) {
+    const NormGradients out =
+        norm_backward(dy, dtotal.value_or(at::Tensor()), normalised, weight.value_or(at::Tensor()), statistics, shape, weight_type, wanted);
     variable_list list = {out.input, out.weight, out.bias};
     for (auto& t : list)
       if (!t.defined()) t = at::empty({0}, normalised.options());
@@ -350,27 +349,26 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
     const at::Tensor residual = residual_.value_or(at::Tensor()), weight = weight_.value_or(at::Tensor()), bias = bias_.value_or(at::Tensor());
     const NormOutputs out = norm_forward(input, residual, weight, bias, shape, eps, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({residual.defined() ? out.total : input, weight, out.mean, out.rstd});
-    ctx->saved_data["dims"] = shape.dims;
-    ctx->saved_data["width"] = shape.width;
-    ctx->saved_data["rows"] = shape.rows;
-    ctx->saved_data["residual"] = residual.defined();
-    ctx->saved_data["bias_dtype"] = bias.defined() ? (int64_t)bias.scalar_type() : int64_t(-1);
+    ctx->save_for_backward({residual.defined() ? out.total : input, weight, out.statistics});
+    const int64_t bias_dtype = bias.defined() ? (int64_t)bias.scalar_type() : int64_t(-1);
+    ctx->saved_data["sizes"] = std::vector<int64_t>{shape.dims, shape.width, shape.rows, residual.defined(), bias_dtype};
     if (residual.defined()) return {out.output, out.total};
     return {out.output};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &normalised = saved[0], &weight = saved[1], &mean = saved[2], &rstd = saved[3];
-    const NormShape shape{ctx->saved_data["dims"].toInt(), ctx->saved_data["width"].toInt(), ctx->saved_data["rows"].toInt()};
-    const int64_t bias_dtype = ctx->saved_data["bias_dtype"].toInt();
+    const at::Tensor &normalised = saved[0], &weight = saved[1], &statistics = saved[2];
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const NormShape shape{sizes[0], sizes[1], sizes[2]};
+    const bool residual = sizes[3] != 0;
+    const int64_t bias_dtype = sizes[4];
     const at::Tensor& dy = grads[0];
     const at::Tensor dtotal = grads.size() > 1 ? grads[1] : at::Tensor();
     // (inputs that were not given have no number here)
     size_t input = 0;
     const bool wants_x = ctx->needs_input_grad(input++);
-    const bool wants_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(input++);
+    const bool wants_r = residual && ctx->needs_input_grad(input++);
     const bool wants_w = weight.defined() && ctx->needs_input_grad(input++);
     const bool wants_b = bias_dtype >= 0 && ctx->needs_input_grad(input++);
     NormGradients out;
@@ -381,10 +379,10 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
           weight.defined() ? weight.scalar_type() : bias_dtype >= 0 ? (at::ScalarType)bias_dtype : normalised.scalar_type();
       const Wanted wanted{wants_x || wants_r, wants_w, wants_b};
       if (at::GradMode::is_enabled()) {
-        const variable_list list = LayerNormBackward::apply(dy, optional(dtotal), normalised, optional(weight), mean, rstd, shape, weight_type, wanted);
+        const variable_list list = LayerNormBackward::apply(dy, optional(dtotal), normalised, optional(weight), statistics, shape, weight_type, wanted);
         out = {list[0], list[1], list[2]};
       } else {
-        out = norm_backward(dy, dtotal, normalised, weight, mean, rstd, shape, weight_type, wanted);
+        out = norm_backward(dy, dtotal, normalised, weight, statistics, shape, weight_type, wanted);
       }
     }
     const auto given = [](bool wanted, const at::Tensor& t) { return wanted ? t : at::Tensor(); };
