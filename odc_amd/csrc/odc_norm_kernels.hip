@@ -12,7 +12,8 @@ using namespace odc_ops_launch;
 // ------------------------------------------------------------------------------------------------
 // kElems neighbouring elements of a row from element i on; what lies behind the row's end is zero, and neither read
 // nor written. kAccess says how:
-// kPlainRows: at any alignment, the piece at the row's end element by element;
+// kPlainRows: at any alignment. A piece that reaches over the row's end is read so that it ends with the row, which needs
+// no branch around the loads, and the elements in front of its own are taken for zeros (rows have a whole piece at least);
 // kBufferRows: rows start at multiples of 16 bytes and end with a whole piece, and all lanes agree on the row. It is a
 // buffer of its own to the hardware, whose bounds check takes the place of branches around the accesses (with them the
 // passes over 16384 x 14336 bf16 took 368 and 691 us instead of 333 and 379);
@@ -30,12 +31,30 @@ struct Piece {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k)
         v[k] = __builtin_bit_cast(typename Vector<T>::type, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(buffer, i * sizeof(T) + k * 16, 0, kPolicy));
-    } else if (i + kElems <= width) {
+    } else if (width) {
+      const uint32_t from = min(i, width - kElems);
 #pragma unroll
-      for (int k = 0; k < kVectors; ++k) v[k] = *reinterpret_cast<const typename Vector<T>::unaligned*>(row + i + k * Vector<T>::kElems);
+      for (int k = 0; k < kVectors; ++k) v[k] = *reinterpret_cast<const typename Vector<T>::unaligned*>(row + from + k * Vector<T>::kElems);
     } else {
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) set(e, i + e < width ? row[i + e] : (T)0.0f);
+      for (int e = 0; e < kElems; ++e) set(e, (T)0.0f);
+    }
+  }
+  // Behind load: element e of the piece is element i + e of the row.
+  __device__ __forceinline__ void settle(uint32_t i, uint32_t width) {
+    if constexpr (kAccess == kPlainRows) {
+      const uint32_t over = i - min(i, width - kElems);  // elements in front of the piece's own
+      if (over) {
+        // one after the other, each by the one `over` places on
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) {
+          T x = (T)0.0f;
+#pragma unroll
+          for (int f = e; f < kElems; ++f)
+            if ((uint32_t)f == e + over) x = v[f / Vector<T>::kElems][f % Vector<T>::kElems];
+          set(e, x);
+        }
+      }
     }
   }
   __device__ __forceinline__ void store(T* row, uint32_t i, uint32_t width) const {
@@ -107,12 +126,14 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
     const uint32_t i = (k * kLanes + lane) * kElems;
     if (c.weight) {
       weight[k].load(static_cast<const W*>(c.weight), i, width);
+      weight[k].settle(i, width);
     } else {
 #pragma unroll
       for (int e = 0; e < kElems; ++e) weight[k].set(e, (W)1.0f);
     }
     if (c.bias) {
       bias[k].load(static_cast<const W*>(c.bias), i, width);
+      bias[k].settle(i, width);
     } else {
 #pragma unroll
       for (int e = 0; e < kElems; ++e) bias[k].set(e, (W)0.0f);
@@ -133,6 +154,11 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
   if constexpr (kAhead) load_row(x);
   while (row < c.rows) {
     if constexpr (!kAhead) load_row(x);
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      x[k].settle((k * kLanes + lane) * kElems, width);
+      if constexpr (kAdd) r[k].settle((k * kLanes + lane) * kElems, width);
+    }
     if constexpr (kAdd) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) {
@@ -183,8 +209,8 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 // grad_input and keeps the sums for weight and bias of its lanes' columns in registers; at the end the rows that it had
 // at once are added in LDS, upper half onto lower half, and go to its row of the workspace.
 template <class T, class W, int kLanes, int kVectors, RowAccess kAccess>
-__global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_backward_kernel(odc_norm_backward c) {
-  constexpr int kThreads = backward_threads({kLanes, kVectors}), kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
+__global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_norm_backward c) {
+  constexpr int kThreads = kBackwardThreads, kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
   constexpr int kSums = 2 * kVectors * kElems;  // of a thread
   __shared__ float scratch[2][2 * kThreads / 64];
   __shared__ float upper[kRows > 1 ? kThreads / 2 * kSums : 1];
@@ -203,6 +229,7 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
     Weight w;
     if (c.weight) {
       w.load(static_cast<const W*>(c.weight), (k * kLanes + lane) * kElems, width);
+      w.settle((k * kLanes + lane) * kElems, width);
     } else {
 #pragma unroll
       for (int e = 0; e < kElems; ++e) w.set(e, (W)1.0f);
@@ -222,33 +249,50 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
     return w;
   };
   int parity = 0;
-  uint64_t row = (uint64_t)blockIdx.x * kRows + slot;
-  Piece<kElems, T, kAccess> x[kVectors], dy[kVectors], dt[kVectors];
-  float mean, rstd;
-  const auto load = [&](Piece<kElems, T, kAccess>(&piece)[kVectors], const void* rows, uint64_t stride) {
+  struct Row {
+    Piece<kElems, T, kAccess> x[kVectors], dy[kVectors], dt[kVectors];
+    float mean, rstd;
+  };
+  const auto load = [&](Piece<kElems, T, kAccess>(&piece)[kVectors], const void* rows, uint64_t stride, uint64_t row) {
 #pragma unroll
     for (int k = 0; k < kVectors; ++k)
       piece[k].load(static_cast<const T*>(rows) + row * stride, (k * kLanes + lane) * kElems, row < c.rows && rows ? width : 0);
   };
-  const auto load_row = [&]() {
-    load(dy, c.grad_output, c.grad_output_stride);
-    load(x, c.normalised, c.normalised_stride);
-    mean = row < c.rows ? c.mean[row] : 0;
-    rstd = row < c.rows ? c.rstd[row] : 0;
+  const auto load_total = [&](Row& r, uint64_t row) {
+    if (c.grad_input) load(r.dt, c.grad_total, c.grad_total_stride, row);
   };
-  // Where registers allow, the next row is on its way while this one's sums are made.
-  constexpr bool kAhead = kAccess != kPlainRows || kVectors == 1;
-  if constexpr (kAhead) load_row();
+  const auto load_row = [&](Row& r, uint64_t row) {
+    load(r.dy, c.grad_output, c.grad_output_stride, row);
+    load(r.x, c.normalised, c.normalised_stride, row);
+    r.mean = row < c.rows ? c.mean[row] : 0;
+    r.rstd = row < c.rows ? c.rstd[row] : 0;
+  };
+  // Rows on their way while one's sums are made, as far as registers go: with 16 wavefronts on a CU, 32 bytes to a lane and
+  // row, one row ahead is half of what keeps HBM busy.
+  constexpr int kAhead = kVectors == 1 ? kRowsAhead : kVectors == 2 && kAccess != kPlainRows ? 1 : 0;
+  constexpr bool kTotalAhead = kVectors == 1;
+  const uint64_t step = (uint64_t)gridDim.x * kRows;
+  Row ring[kAhead + 1];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    load_row(ring[a], (uint64_t)blockIdx.x * kRows + slot + a * step);
+    if constexpr (kTotalAhead) load_total(ring[a], (uint64_t)blockIdx.x * kRows + slot + a * step);
+  }
   // every thread makes the same number of rounds: there are barriers in them
-  for (uint64_t first = (uint64_t)blockIdx.x * kRows; first < c.rows; first += (uint64_t)gridDim.x * kRows, parity ^= 1) {
-    if constexpr (!kAhead) load_row();
+  for (uint64_t first = (uint64_t)blockIdx.x * kRows; first < c.rows; first += step, parity ^= 1) {
+    const uint64_t row = first + slot;
+    const bool mine = row < c.rows;
+    Row& r = ring[0];
+    if constexpr (kAhead == 0) load_row(r, row);
     float row_sum[2] = {};
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
+      r.x[k].settle((k * kLanes + lane) * kElems, width);
+      r.dy[k].settle((k * kLanes + lane) * kElems, mine ? width : 0);
       const Weight w = weight(k);
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
-        const float z = (x[k][e] - mean) * rstd, g = dy[k][e];  // behind the row's end g is zero and z of no account
+        const float z = (r.x[k][e] - r.mean) * r.rstd, g = r.dy[k][e];  // behind the row's end g is zero and z of no account
         const float h = g * w[e];
         row_sum[0] += h;
         row_sum[1] += h * z;
@@ -257,33 +301,33 @@ __global__ __launch_bounds__(backward_threads({kLanes, kVectors})) void norm_bac
       }
       if constexpr (kVectors > 1) __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time: registers
     }
-    const uint64_t here = row;
-    const float mean_here = mean, rstd_here = rstd;
-    Piece<kElems, T, kAccess> x_here[kVectors], dy_here[kVectors];
-#pragma unroll
-    for (int k = 0; k < kVectors; ++k) x_here[k] = x[k], dy_here[k] = dy[k];
-    if (c.grad_input) load(dt, c.grad_total, c.grad_total_stride);
-    row += (uint64_t)gridDim.x * kRows;
-    if constexpr (kAhead) load_row();
+    if constexpr (!kTotalAhead) load_total(r, row);
+    if constexpr (kAhead > 0) {
+      load_row(ring[kAhead], row + kAhead * step);
+      if constexpr (kTotalAhead) load_total(ring[kAhead], row + kAhead * step);
+    }
     if (c.grad_input) {
       row_sums<kLanes>(row_sum, scratch[parity]);
       const float sum = row_sum[0] * per_element, dot = row_sum[1] * per_element;
-      if (here < c.rows) {
+      if (mine) {
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
-          x_here[k].forget();
-          dy_here[k].forget();
+          r.x[k].forget();
+          r.dy[k].forget();
+          if (c.grad_total) r.dt[k].settle((k * kLanes + lane) * kElems, width);
           const Weight w = weight(k);
 #pragma unroll
           for (int e = 0; e < kElems; ++e) {
-            const float z = (x_here[k][e] - mean_here) * rstd_here, h = dy_here[k][e] * w[e];
-            x_here[k].set(e, from_float<T>(rstd_here * (h - sum - z * dot) + dt[k][e]));
+            const float z = (r.x[k][e] - r.mean) * r.rstd, h = r.dy[k][e] * w[e];
+            r.x[k].set(e, from_float<T>(r.rstd * (h - sum - z * dot) + r.dt[k][e]));
           }
-          x_here[k].store(static_cast<T*>(c.grad_input) + here * c.width, (k * kLanes + lane) * kElems, width);
+          r.x[k].store(static_cast<T*>(c.grad_input) + row * c.width, (k * kLanes + lane) * kElems, width);
           if constexpr (kVectors > 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) ring[a] = ring[a + 1];
   }
   if (!sums) return;
 #pragma unroll
@@ -523,12 +567,14 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
     hipStream_t s = (hipStream_t)stream;
     const bool sums = call.grad_weight || call.grad_bias;
     if (plan.shape.lanes && plan.groups) {
-      with_shape<kBackwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
+      const auto launch = [&](auto lanes, auto vectors) {
         constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
         with_access<kLanes>(plan.access, [&](auto access) {
-          norm_backward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value><<<plan.groups, backward_threads(plan.shape), 0, s>>>(call);
+          norm_backward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value><<<plan.groups, kBackwardThreads, 0, s>>>(call);
         });
-      });
+      };
+      if constexpr (sizeof(T) == 4) with_shape<kBackwardShapes32>(plan.shape, launch);
+      else with_shape<kBackwardShapes16>(plan.shape, launch);
     } else if (plan.groups) {
       if (call.grad_input) norm_backward_rows_kernel<T, W><<<plan.row_blocks, kWideThreads, 0, s>>>(call);
       const uint32_t tiles = (uint32_t)((call.width + kColumnTile - 1) / kColumnTile);

@@ -104,10 +104,10 @@ NormForwardPlan forward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
 
 NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
   NormBackwardPlan plan = {};
-  plan.shape = shape_of(kBackwardShapes, width, dtype);
+  plan.shape = dtype == ODC_OPS_F32 ? shape_of(kBackwardShapes32, width, dtype) : shape_of(kBackwardShapes16, width, dtype);
   plan.row_blocks = (uint32_t)std::min<uint64_t>(rows, 8 * kCus);
   if (plan.shape.lanes) {
-    plan.groups = (uint32_t)std::min(ceil_div(rows, backward_threads(plan.shape) / plan.shape.lanes), kCus);
+    plan.groups = (uint32_t)std::min(ceil_div(rows, kBackwardThreads / plan.shape.lanes), kCus);
     plan.rows_per_group = 0;
   } else {
     plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kCus));

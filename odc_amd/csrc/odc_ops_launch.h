@@ -18,19 +18,26 @@ inline uint32_t bytes_of(int32_t dtype) { return dtype == ODC_OPS_F32 ? 4 : 2; }
 
 // ---- layer norm -----------------------------------------------------------------------------------
 // A row is held in the registers of `lanes` lanes, `vectors` vectors of 16 bytes each; rows wider than the last shape
-// are passed over three times.
+// are passed over three times. The backward pass has sums for weight and bias beside them, 16 or 8 registers to a vector.
 struct NormShape {
   uint32_t lanes, vectors;
 };
 constexpr NormShape kForwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}, {1024, 4}};
-constexpr NormShape kBackwardShapes[] = {{16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}};
-constexpr uint32_t kForwardThreads = 256;    // of a workgroup; where a row takes more lanes, as many as those
-constexpr uint32_t backward_threads(NormShape) { return 1024; }
-constexpr uint32_t kWideThreads = 256;       // of one for wide rows
+constexpr NormShape kBackwardShapes16[] = {{16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}};
+constexpr NormShape kBackwardShapes32[] = {{16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+constexpr uint32_t kForwardThreads = 256;  // of a workgroup; where a row takes more lanes, as many as those
+// One workgroup to a CU: each writes its sums of all columns, and a second launch reads them. (Two of 512 threads: level
+// for long passes, 33.8 instead of 32.0 us for 4096 x 4096.)
+constexpr uint32_t kBackwardThreads = 1024;
+constexpr uint32_t kWideThreads = 256;  // of one for wide rows
+// Rows ahead of the one that a backward pass works on, with one vector to a lane. us for 16384 x 4096 bf16 with 1, 2, 3:
+// 86.5, 74.2, 75.9; 65536 x 1024: 82.6, 69.8, 70.7.
+constexpr int kRowsAhead = 2;
 
-// The first of `shapes` that holds a row; lanes 0: none does.
+// The first of `shapes` that holds a row; lanes 0: none does, or the row is less than a vector.
 template <size_t n>
 inline NormShape shape_of(const NormShape (&shapes)[n], uint64_t width, int32_t dtype) {
+  if (width < 16 / bytes_of(dtype)) return {0, 0};
   for (const NormShape& s : shapes)
     if (width <= (uint64_t)s.lanes * s.vectors * (16 / bytes_of(dtype))) return s;
   return {0, 0};
