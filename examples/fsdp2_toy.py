@@ -9,7 +9,12 @@ microbatches -> ``pre_optimizer_step`` -> optimizer). Where that script compares
 between runs (``examples/FSDP2/utils.py:29-66``), this one keeps an unsharded copy of the model
 in the same process and checks rank 0's gradient shards against it bit for bit at every step.
 
+``--native-ops`` computes the norms, the residual additions in front of them and the optimizer step by the package's own
+operators (``odc_amd.ops``): ``LayerNorm``, ``AdamW`` with states in 32 bits or 8 (``--state-bits 8``) and clipping by the
+norm of all gradients. The twin runs the same norms, and the gradient shards match it bit for bit as before.
+
     python examples/fsdp2_toy.py [--world-size 8] [--mixed-precision] [--explicit-prefetching]
+    python examples/fsdp2_toy.py --native-ops [--state-bits 8] [--mixed-precision]
 """
 
 from __future__ import annotations
@@ -30,13 +35,14 @@ sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 
 class Block(nn.Module):
-    def __init__(self, dim, heads):
+    def __init__(self, dim, heads, norm=nn.LayerNorm):
         super().__init__()
         self.heads = heads
-        self.norm1 = nn.LayerNorm(dim)
+        self.fused = norm is not nn.LayerNorm  # odc_amd.ops.LayerNorm takes a residual
+        self.norm1 = norm(dim)
         self.qkv = nn.Linear(dim, 3 * dim, bias=False)
         self.proj = nn.Linear(dim, dim, bias=False)
-        self.norm2 = nn.LayerNorm(dim)
+        self.norm2 = norm(dim)
         self.up = nn.Linear(dim, 4 * dim)
         self.down = nn.Linear(4 * dim, dim)
 
@@ -48,17 +54,22 @@ class Block(nn.Module):
         scores = (q @ k.transpose(-1, -2)) / math.sqrt(d // self.heads)
         causal = torch.ones(t, t, dtype=torch.bool, device=x.device).tril()
         attn = scores.masked_fill(~causal, float("-inf")).softmax(-1) @ v
-        x = x + self.proj(attn.transpose(1, 2).reshape(b, t, d))
-        return x + self.down(F.gelu(self.up(self.norm2(x))))
+        y = self.proj(attn.transpose(1, 2).reshape(b, t, d))
+        if self.fused:
+            y, x = self.norm2(y, x)  # the residual addition and the norm of its result, in one pass
+        else:
+            x = x + y
+            y = self.norm2(x)
+        return x + self.down(F.gelu(self.up(y)))
 
 
 class ToyLM(nn.Module):
-    def __init__(self, vocab=1024, seq=64, dim=256, heads=4, layers=2):
+    def __init__(self, vocab=1024, seq=64, dim=256, heads=4, layers=2, norm=nn.LayerNorm):
         super().__init__()
         self.tok = nn.Embedding(vocab, dim)
         self.pos = nn.Embedding(seq, dim)
-        self.layers = nn.ModuleList([Block(dim, heads) for _ in range(layers)])
-        self.norm = nn.LayerNorm(dim)
+        self.layers = nn.ModuleList([Block(dim, heads, norm) for _ in range(layers)])
+        self.norm = norm(dim)
         self.out = nn.Linear(dim, vocab, bias=False)
 
     def forward(self, tokens):
@@ -89,6 +100,9 @@ def main():
     ap.add_argument("--sync-every", type=int, default=1,
                     help="reduce gradients only every so many microbatches (set_requires_gradient_sync); in "
                          "between they add up unsharded, in the compute dtype")
+    ap.add_argument("--native-ops", action="store_true", help="norms and optimizer step by odc_amd.ops")
+    ap.add_argument("--state-bits", type=int, choices=[8, 32], default=32, help="with --native-ops: of the AdamW states")
+    ap.add_argument("--max-norm", type=float, default=1.0, help="with --native-ops: clip the gradients to it")
     args = ap.parse_args()
 
     from torch.distributed.device_mesh import init_device_mesh
@@ -107,7 +121,12 @@ def main():
 
     torch.manual_seed(0)
     vocab, seq, batch = 1024, 64, 32
-    model = ToyLM(vocab=vocab, seq=seq, layers=args.layers).cuda()
+    norm = nn.LayerNorm
+    if args.native_ops:
+        from odc_amd import ops
+
+        norm = ops.LayerNorm
+    model = ToyLM(vocab=vocab, seq=seq, layers=args.layers, norm=norm).cuda()
     unsharded = copy.deepcopy(model)
     full_params = {n: p.detach().clone() for n, p in unsharded.named_parameters()}
 
@@ -144,7 +163,10 @@ def main():
         for i, layer in enumerate(model.layers[1:], start=1):
             layer.set_modules_to_backward_prefetch([model.layers[i - 1]])
 
-    optim = torch.optim.Adam(model.parameters(), lr=1e-3)
+    if args.native_ops:
+        optim = ops.AdamW(model.parameters(), lr=1e-3, weight_decay=0.0, state_bits=args.state_bits, max_norm=args.max_norm)
+    else:
+        optim = torch.optim.Adam(model.parameters(), lr=1e-3)
     names = [n for n, _ in model.named_parameters()]
     data = torch.Generator(device="cuda").manual_seed(1)
     t0 = time.perf_counter()
@@ -185,7 +207,12 @@ def main():
             if not torch.equal(got.view(torch.int32), expect.view(torch.int32)):
                 worst = (got - expect).abs().max().item()
                 raise SystemExit(f"step {step}: gradient shard of {n} differs from the unsharded model (max |d| {worst:g})")
-        optim.step()
+        if args.native_ops:
+            # Clipped by the norm of all ranks' gradients, which the twin has whole. With a process for each rank it is
+            # the sum over the ranks of ops.squared_norm of their own shards (one all_reduce of a number).
+            optim.step(squared_norm=ops.squared_norm([want[n].float() / post_divide for n in names]))
+        else:
+            optim.step()
         optim.zero_grad()
         print(f"step {step} loss {loss.item():.4f}  gradient shards match the unsharded model bit for bit")
     torch.cuda.synchronize()

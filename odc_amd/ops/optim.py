@@ -125,6 +125,8 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step cannot be captured into a graph: the step's number would be a constant of it")
+        if squared_norm is not None and self.max_norm is None:
+            raise ValueError("squared_norm without max_norm: there is nothing to clip to")
         calls, sharded = {}, []
         for number, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -139,31 +141,33 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if grad.stride() != param.stride() and not (grad.is_contiguous() and param.is_contiguous()):
                     grad = torch.empty_like(param, dtype=grad.dtype).copy_(grad)
-                state = self.state[p]
-                if not state:
-                    self._begin(state, p, param)
-                state["step"] += 1
-                key = (number, state["step"], param.device, param.dtype, grad.dtype)
-                calls.setdefault(key, []).append((param, grad, state))
+                steps = self.state[p]["step"] if self.state[p] else 0
+                calls.setdefault((number, steps + 1, param.device, param.dtype, grad.dtype), []).append((p, param, grad))
         if squared_norm is None and self.max_norm is not None and calls:
             if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
-            squared_norm = _host_squared_norm([grad for call in calls.values() for _, grad, _ in call])
-        if squared_norm is not None and self.max_norm is None:
-            raise ValueError("squared_norm without max_norm: there is nothing to clip to")
-        for place, ((number, step, device, dtype, _), call) in enumerate(calls.items()):
+            squared_norm = _host_squared_norm([grad for call in calls.values() for _, _, grad in call])
+        for place, ((number, step, device, _, _), call) in enumerate(calls.items()):
             group = self.param_groups[number]
             numbers = dict(step=step, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
                            weight_decay=group["weight_decay"], grad_scale=grad_scale, max_norm=self.max_norm,
                            squared_norm=None if squared_norm is None else squared_norm.to(device))
             # another seed for every step, and for every call of a step
             seed = (self.seed * 0x9E3779B1 + step * 0x85EB + place * 0x27D4EB2F) & 0xFFFFFFFF
-            params, grads, states = zip(*call)
+            states = []
+            for p, param, _ in call:
+                state = self.state[p]
+                if not state:
+                    self._begin(state, p, param)
+                states.append(state)
+            _, params, grads = zip(*call)
             if self.state_bits == 8:
                 adamw_step_8bit(params, grads, *([s[name] for s in states] for name in _STATES_8BIT), seed=seed, **numbers)
             else:
                 adamw_step(params, grads, *([_local(s[name]) for s in states] for name in ("exp_avg", "exp_avg_sq")),
                            seed=seed if self.stochastic_params else None, **numbers)
+            for state in states:
+                state["step"] = step
         if sharded:
             torch.autograd.graph.increment_version(sharded)  # of a DTensor: its local tensor has a counter of its own
         shards_may_have_changed()
