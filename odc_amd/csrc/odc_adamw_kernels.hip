@@ -199,18 +199,17 @@ __device__ __forceinline__ float chosen_value(float x, float inverse_scale, uint
   return __uint_as_float(bits & 0xFFF00000u) - shift;
 }
 
-// Where that of the square is kept: with the codes a and a + s beside t the share is (t - a)(t + a) / (s (2 a + s)).
-// What is not zero does not become zero. `eight` is 8 s, the power of two that t begins with.
-__device__ __forceinline__ float chosen_root(float x, float inverse_scale, uint32_t half) {
+// Where that of the square v = x^2 is kept: with the codes a and a + s beside x the share is (v - a^2) / (s (2 a + s)), made
+// from v itself: the root has been rounded, a's square is exact. What is not zero does not become zero. `eight` is 8 s,
+// the power of two that x begins with.
+__device__ __forceinline__ float chosen_root(float x, float v, float inverse_scale, uint32_t half) {
   float size = x * inverse_scale;
   size = size > 0 ? fmaxf(size, 0x1p-9f) : size;
   const float shift = size < 0x1p-6f ? 0x1p-6f : 0.0f;
-  const float lifted = size + shift;
-  const uint32_t bits = __float_as_uint(lifted);
-  const float below_lifted = __uint_as_float(bits & 0xFFF00000u), eight = __uint_as_float(bits & 0x7F800000u);
-  const float below = below_lifted - shift;
-  const float whole = ((float)half * 0x1p-22f + 0x1p-23f) * eight * (16 * below + eight);  // 64 times s (2 a + s), in 2^-16
-  return whole < (lifted - below_lifted) * (size + below) ? below + 0.125f * eight : below;
+  const uint32_t bits = __float_as_uint(size + shift);
+  const float below = __uint_as_float(bits & 0xFFF00000u) - shift, eight = __uint_as_float(bits & 0x7F800000u);
+  const float whole = ((float)half * 0x1p-22f + 0x1p-23f) * eight * (16 * below + eight);  // (half + 0.5) / 65536 of s (2 a + s)
+  return whole < v * inverse_scale * inverse_scale - below * below ? below + 0.125f * eight : below;
 }
 
 __device__ __forceinline__ float scale_value(uint32_t scale) { return __uint_as_float(scale << 23); }
@@ -223,17 +222,17 @@ __device__ __forceinline__ void values_of(uint32_t codes, float factor, float (&
   x[3] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 3) * factor;
 }
 
-// The codes of four values and the scale of their block. kRoots: roots, by the high halves of the words; else by the
-// low ones.
+// The codes of four values and the scale of their block. kRoots: the roots of `squares`, by the high halves of the words;
+// else any values, by the low ones.
 template <bool kRoots>
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], const uint32_t (&word)[4], uint32_t& scale) {
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[4], const float (&squares)[4], const uint32_t (&word)[4], uint32_t& scale) {
   bool odd;
   scale = scale_of(largest_of(x, odd));
   const float inverse = __uint_as_float((254u - scale) << 23);
   float c[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    c[e] = kRoots ? chosen_root(x[e], inverse, word[e] >> 16) : copysignf(chosen_value(x[e], inverse, word[e] & 0xFFFFu), x[e]);
+    c[e] = kRoots ? chosen_root(x[e], squares[e], inverse, word[e] >> 16) : copysignf(chosen_value(x[e], inverse, word[e] & 0xFFFFu), x[e]);
   const int low = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
   uint32_t codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], low, true);
   if (odd) {
@@ -248,20 +247,20 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], const uint32_t
 // kVectors times four elements to a lane, all of their loads before the first store; `elems` from element `first` on.
 template <class P, class G, class C, bool kEight, bool kStream, bool kWhole>
 __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k, uint64_t first, uint32_t elems) {
-  const odc_adamw_item& it = launch.items[k];
   constexpr AdamwShape kShape = adamw_shape(kEight);
   constexpr uint32_t kThreads = kShape.threads, kVectors = kShape.vectors;
   const float factor = factor_of(launch);
   const bool stochastic = sizeof(P) == 2 && launch.stochastic;
   const uint32_t key = kEight || stochastic ? mix(launch.seed + (launch.first_item + k) * 0x9E3779B1u) : 0;
-  P* const param = static_cast<P*>(it.param) + first;
-  const G* const grad = static_cast<const G*>(it.grad) + first;
-  C* const copy = it.copy ? static_cast<C*>(it.copy) + first : nullptr;
+  const uint64_t* const words = launch.words + k * launch.words_per_item + 1;  // (AdamwLaunch::set)
+  P* const param = reinterpret_cast<P*>(words[0]) + first;
+  const G* const grad = reinterpret_cast<const G*>(words[1]) + first;
   typedef std::conditional_t<kEight, uint8_t, float> S;
-  S* const m_state = static_cast<S*>(it.exp_avg) + first;
-  S* const v_state = static_cast<S*>(it.exp_avg_sq) + first;
-  uint8_t* const m_scale = static_cast<uint8_t*>(it.exp_avg_scale) + first / kBlock;
-  uint8_t* const v_scale = static_cast<uint8_t*>(it.exp_avg_sq_scale) + first / kBlock;
+  S* const m_state = reinterpret_cast<S*>(words[2]) + first;
+  S* const v_state = reinterpret_cast<S*>(words[3]) + first;
+  uint8_t* const m_scale = kEight ? reinterpret_cast<uint8_t*>(words[4]) + first / kBlock : nullptr;
+  uint8_t* const v_scale = kEight ? reinterpret_cast<uint8_t*>(words[5]) + first / kBlock : nullptr;
+  C* const copy = launch.words_per_item % 2 == 0 ? reinterpret_cast<C*>(words[kEight ? 6 : 4]) + first : nullptr;
   Four<P> p[kVectors];
   Four<G> g[kVectors];
   Four<S> m[kVectors], v[kVectors];
@@ -308,8 +307,8 @@ __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k
       }
     }
     if constexpr (kEight) {  // (lanes without elements hold zeros, and come along to their block's largest value)
-      m[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<false>(m_now, word, m_exponent[u]));
-      v[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<true>(root, word, v_exponent[u]));
+      m[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<false>(m_now, v_now, word, m_exponent[u]));
+      v[u].v = __builtin_bit_cast(typename Four<S>::type, codes_of<true>(root, v_now, word, v_exponent[u]));
       if (n && threadIdx.x % (kBlock / 4) == 0) {
         m_scale[i / kBlock] = (uint8_t)m_exponent[u];
         v_scale[i / kBlock] = (uint8_t)v_exponent[u];
@@ -327,7 +326,7 @@ __global__ __launch_bounds__(adamw_shape(kEight).threads) __attribute__((amdgpu_
     AdamwLaunch launch) {
   constexpr uint32_t kTile = adamw_shape(kEight).tile();
   const uint32_t k = item_of(launch, blockIdx.x);
-  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kTile, left = launch.items[k].elems - first;
+  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kTile, left = launch.words[k * launch.words_per_item] - first;
   if (left >= kTile) adamw_tile<P, G, C, kEight, kStream, true>(launch, k, first, kTile);
   else adamw_tile<P, G, C, kEight, kStream, false>(launch, k, first, (uint32_t)left);
 }

@@ -201,16 +201,16 @@ int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {
   return launched(odc_ops_device::launch_norm_backward(c, plan, stream));
 }
 
+// A partial sum for every workgroup: as many as tiles, at most kMostPartials for each launch.
 uint64_t odc_squared_norm_workspace(const odc_span_item* items, uint32_t n_items, int32_t dtype) {
   if (!items || !is_float_type(dtype)) return 0;
-  uint64_t partials = 0;
-  SquaredNormLaunch launch;
-  for (uint32_t at = 0; at < n_items;) {
-    if (check_elems(items[at].elems, at, kNormTile, kNormThreads) != ODC_OPS_OK) return 0;
-    at = fill_table(launch, items, n_items, at, kNormItems, kNormTile, kNormThreads);
-    partials += partials_of(launch.n_tiles);
+  uint64_t tiles = 0;
+  for (uint32_t i = 0; i < n_items; ++i) {
+    if (check_elems(items[i].elems, i, kNormTile, kNormThreads) != ODC_OPS_OK) return 0;
+    tiles += ceil_div(items[i].elems, kNormTile);
   }
-  return partials * sizeof(double);
+  const uint64_t launches = ceil_div(n_items, kNormItems) + 2 * (tiles / most_workgroups(kNormThreads));
+  return std::min(tiles, launches * kMostPartials) * sizeof(double);
 }
 
 int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype, void* workspace, uint64_t workspace_bytes, float* result,
@@ -286,9 +286,10 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
   launch.squared_norm = a.squared_norm;
   launch.seed = a.seed;
   launch.stochastic = a.stochastic != 0;
+  launch.words_per_item = AdamwLaunch::words_of(a.state_bits == 8, a.copy_dtype != ODC_OPS_NONE);
   for (uint32_t at = 0; at < n_items;) {
     launch.first_item = at;
-    at = fill_table(launch, items, n_items, at, kAdamwItems, shape.tile(), shape.threads);
+    at = fill_table(launch, items, n_items, at, kAdamwWords / launch.words_per_item, shape.tile(), shape.threads);
     if (!launch.n_tiles) continue;
     ODC_OPS_TRY(launched(odc_ops_device::launch_adamw(a.param_dtype, a.grad_dtype, a.copy_dtype, a.state_bits, past_caches, launch, stream)));
   }

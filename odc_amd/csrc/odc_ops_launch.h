@@ -87,7 +87,6 @@ struct SquaredNormLaunch {
 static_assert(sizeof(SquaredNormLaunch) <= 3900, "kernel arguments are limited to 4 KiB");
 
 constexpr uint32_t kBlock = 32;  // elements of a state in 8 bits that share a scale
-constexpr uint32_t kAdamwItems = 48;
 // A workgroup of the AdamW step: its threads, how many vectors of four elements a lane has, and how many wavefronts a SIMD
 // may hold (a bound in the kernel's own attributes).
 struct AdamwShape {
@@ -100,6 +99,7 @@ struct AdamwShape {
 // 256 threads 4897 / 139; two vectors to a lane 5143 / 142. States in 8 bits have arithmetic to hide, about 70 instructions for
 // an element: 256 threads x 2 144, x 1 148, 64 x 2 147 us over 27 M with clipping.
 constexpr AdamwShape adamw_shape(bool eight) { return eight ? AdamwShape{256, 2, 8} : AdamwShape{64, 1, 3}; }
+constexpr uint32_t kAdamwWords = 400;
 struct AdamwLaunch {
   float beta1, beta2, one_minus_beta1, one_minus_beta2;
   float decay;          // 1 - lr * weight_decay
@@ -109,12 +109,24 @@ struct AdamwLaunch {
   const float* squared_norm;
   uint32_t seed, first_item, stochastic;
   uint32_t n_items, n_tiles;
-  uint32_t first_tile[kAdamwItems + 1];
-  odc_adamw_item items[kAdamwItems];
+  // An item takes the words that it needs: five pointers or six with a copy, of states in 8 bits two more for the scales. So
+  // a launch has room for 80, 66, 57 or 50 of them (a launch costs the host about 3 us).
+  uint32_t words_per_item;
+  uint32_t first_tile[kAdamwWords / 5 + 1];
+  uint64_t words[kAdamwWords];
 
-  void set(uint32_t k, const odc_adamw_item& item) { items[k] = item; }
+  static uint32_t words_of(bool eight, bool copies) { return 5 + copies + 2 * eight; }
+  void set(uint32_t k, const odc_adamw_item& item) {
+    uint64_t* w = words + k * words_per_item;
+    const void* const pointers[] = {item.param, item.grad, item.exp_avg, item.exp_avg_sq};
+    *w++ = item.elems;
+    for (const void* p : pointers) *w++ = (uint64_t)(uintptr_t)p;
+    const bool eight = words_per_item >= 7, copies = words_per_item % 2 == 0;
+    if (eight) *w++ = (uint64_t)(uintptr_t)item.exp_avg_scale, *w++ = (uint64_t)(uintptr_t)item.exp_avg_sq_scale;
+    if (copies) *w++ = (uint64_t)(uintptr_t)item.copy;
+  }
 };
-static_assert(sizeof(AdamwLaunch) <= 3800, "kernel arguments are limited to 4 KiB");
+static_assert(sizeof(AdamwLaunch) <= 3900, "kernel arguments are limited to 4 KiB");
 
 }  // namespace odc_ops_launch
 

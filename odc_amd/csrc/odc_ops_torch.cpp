@@ -160,7 +160,9 @@ void expect_gpu(const char* what, const at::Tensor& t) {
   if (!t.is_cuda() || t.layout() != at::kStrided) raise(PyExc_TypeError, "%s: expected a dense tensor on the GPU", what);
 }
 
+// `device` is a GPU. (A tensor that is not dense has no data pointer: asking for it raises.)
 void expect_device(const char* what, const at::Tensor& t, const at::Device& device) {
+  if (t.device() == device) return;
   expect_gpu(what, t);
   if (t.device() != device) raise(PyExc_ValueError, "%s is on %s, not on %s", what, t.device().str().c_str(), device.str().c_str());
 }
@@ -502,6 +504,7 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+  if (a.dim() == 1 && b.dim() == 1) return a.numel() == b.numel() && a.is_contiguous() && b.is_contiguous();
   return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
 }
 
@@ -618,7 +621,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
       items.push_back(item);
       if (numel) spans.emplace_back((uintptr_t)item.param, (uintptr_t)item.param + (uintptr_t)numel * p.element_size());
     }
-    std::sort(spans.begin(), spans.end());
+    if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());  // (the allocator's order, as a rule)
     for (size_t k = 1; k < spans.size(); ++k)
       if (spans[k].first < spans[k - 1].second) raise(PyExc_ValueError, "params: two tensors overlap");
     numbers.param_dtype = float_code("params", first);

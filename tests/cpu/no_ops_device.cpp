@@ -55,7 +55,15 @@ namespace {
 // Made-up device addresses: nothing here reads through them.
 void* at(uintptr_t address) { return reinterpret_cast<void*>(address); }
 
-void check_item(const AdamwLaunch& launch, uint32_t i, const odc_adamw_item& item) { CHECK(launch.items[i].elems == item.elems); }
+void check_item(const AdamwLaunch& launch, uint32_t i, const odc_adamw_item& item) {
+  const uint64_t* w = launch.words + i * launch.words_per_item;
+  const auto is = [](uint64_t word, const void* p) { return word == (uint64_t)(uintptr_t)p; };
+  CHECK((i + 1) * launch.words_per_item <= kAdamwWords);
+  CHECK(w[0] == item.elems && is(w[1], item.param) && is(w[2], item.grad) && is(w[3], item.exp_avg) && is(w[4], item.exp_avg_sq));
+  const uint32_t scales = launch.words_per_item >= 7 ? 2 : 0;
+  CHECK(!scales || (is(w[5], item.exp_avg_scale) && is(w[6], item.exp_avg_sq_scale)));
+  CHECK(launch.words_per_item == 5 + scales + (item.copy != nullptr) && (!item.copy || is(w[5 + scales], item.copy)));
+}
 void check_item(const SquaredNormLaunch& launch, uint32_t i, const odc_span_item& item) {
   const uint64_t tiles = launch.first_tile[i + 1] - launch.first_tile[i], last = launch.places[i] & 0xFFFF;
   CHECK(launch.places[i] >> 16 == (uint64_t)(uintptr_t)item.data && (tiles ? (tiles - 1) * kNormTile + last : 0) == item.elems);
@@ -156,16 +164,19 @@ void check_lists() {
     float result;
     CHECK(odc_squared_norm(spans.data(), (uint32_t)spans.size(), ODC_OPS_BF16, workspace.data(), bytes, &result, nullptr) == ODC_OPS_OK);
     check_tables(seen.squared, spans, kNormTile);
-    CHECK(seen.totals == 1 && seen.total_partials * sizeof(double) == bytes);
+    CHECK(seen.totals == 1 && seen.total_partials * sizeof(double) <= bytes);
     uint64_t done = 0;
     for (size_t k = 0; k < seen.squared.size(); ++k) {
       CHECK(seen.squared_partials[k] == workspace.data() + done && seen.squared_blocks[k] > 0 && seen.squared_blocks[k] <= seen.squared[k].n_tiles);
       done += seen.squared_blocks[k];
     }
     if (bytes) CHECK(odc_squared_norm(spans.data(), (uint32_t)spans.size(), ODC_OPS_BF16, workspace.data(), bytes - 8, &result, nullptr) < 0);
-    for (int bits : {8, 32}) {
+    for (int form = 0; form < 4; ++form) {
+      const int bits = form % 2 ? 8 : 32;
       seen = Seen();
       odc_adamw_numbers a = {1e-3, 0.9, 0.999, 1e-8, 0.1, 1.0, 0.0, nullptr, 3, 7, 0, ODC_OPS_F32, ODC_OPS_BF16, ODC_OPS_NONE, bits};
+      a.copy_dtype = form < 2 ? ODC_OPS_NONE : ODC_OPS_BF16;
+      for (odc_adamw_item& item : items) item.copy = form < 2 ? nullptr : at(0x7000);
       CHECK(odc_adamw(items.data(), (uint32_t)items.size(), &a, nullptr) == ODC_OPS_OK);
       check_tables(seen.adamw, items, adamw_shape(bits == 8).tile());
       uint32_t first = 0;
