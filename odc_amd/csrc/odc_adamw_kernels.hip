@@ -245,6 +245,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], const float (&
 
 // ---- the step -------------------------------------------------------------------------------------
 // kVectors times four elements to a lane, all of their loads before the first store; `elems` from element `first` on.
+// C: the type of copies, or void where there are none.
 template <class P, class G, class C, bool kEight, bool kStream, bool kWhole>
 __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k, uint64_t first, uint32_t elems) {
   constexpr AdamwShape kShape = adamw_shape(kEight);
@@ -252,7 +253,9 @@ __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k
   const float factor = factor_of(launch);
   const bool stochastic = sizeof(P) == 2 && launch.stochastic;
   const uint32_t key = kEight || stochastic ? mix(launch.seed + (launch.first_item + k) * 0x9E3779B1u) : 0;
-  const uint64_t* const words = launch.words + k * launch.words_per_item + 1;  // (AdamwLaunch::set)
+  constexpr bool kCopies = !std::is_void_v<C>;
+  typedef std::conditional_t<kCopies, C, bf16> Copy;
+  const uint64_t* const words = launch.words + k * AdamwLaunch::words_of(kEight, kCopies) + 1;  // (AdamwLaunch::set)
   P* const param = reinterpret_cast<P*>(words[0]) + first;
   const G* const grad = reinterpret_cast<const G*>(words[1]) + first;
   typedef std::conditional_t<kEight, uint8_t, float> S;
@@ -260,7 +263,7 @@ __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k
   S* const v_state = reinterpret_cast<S*>(words[3]) + first;
   uint8_t* const m_scale = kEight ? reinterpret_cast<uint8_t*>(words[4]) + first / kBlock : nullptr;
   uint8_t* const v_scale = kEight ? reinterpret_cast<uint8_t*>(words[5]) + first / kBlock : nullptr;
-  C* const copy = launch.words_per_item % 2 == 0 ? reinterpret_cast<C*>(words[kEight ? 6 : 4]) + first : nullptr;
+  Copy* const copy = kCopies ? reinterpret_cast<Copy*>(words[kEight ? 6 : 4]) + first : nullptr;
   Four<P> p[kVectors];
   Four<G> g[kVectors];
   Four<S> m[kVectors], v[kVectors];
@@ -295,12 +298,15 @@ __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k
       if (kEight || stochastic) word[e] = word_of(first + i + e, key);
     }
     roots_of(v_now, root);
-    Four<C> c;
+    Four<Copy> c;
 #pragma unroll
     for (uint32_t e = 0; e < 4; ++e) {
-      const float q = next_param(launch, to_float(p[u].v[e]), m_now[e], root[e]);
+      float q = next_param(launch, to_float(p[u].v[e]), m_now[e], root[e]);
+      // The copy is the parameter's rounding: the compiler would make it of the unrounded difference, by an instruction
+      // that subtracts into fp16.
+      if constexpr (kCopies) asm("" : "+v"(q));
       p[u].v[e] = stored_param<P>(q, stochastic, word[e]);
-      c.v[e] = from_float<C>(q);
+      c.v[e] = from_float<Copy>(q);
       if constexpr (!kEight) {
         m[u].v[e] = m_now[e];
         v[u].v[e] = v_now[e];
@@ -317,7 +323,7 @@ __device__ __forceinline__ void adamw_tile(const AdamwLaunch& launch, uint32_t k
     p[u].template store<kStream>(param + i, n);
     m[u].template store<kStream>(m_state + i, n);
     v[u].template store<kStream>(v_state + i, n);
-    if (copy) c.template store<false>(copy + i, n);
+    if constexpr (kCopies) c.template store<false>(copy + i, n);
   }
 }
 
@@ -326,7 +332,7 @@ __global__ __launch_bounds__(adamw_shape(kEight).threads) __attribute__((amdgpu_
     AdamwLaunch launch) {
   constexpr uint32_t kTile = adamw_shape(kEight).tile();
   const uint32_t k = item_of(launch, blockIdx.x);
-  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kTile, left = launch.words[k * launch.words_per_item] - first;
+  const uint64_t first = (uint64_t)(blockIdx.x - launch.first_tile[k]) * kTile, left = launch.words[k * AdamwLaunch::words_of(kEight, !std::is_void_v<C>)] - first;
   if (left >= kTile) adamw_tile<P, G, C, kEight, kStream, true>(launch, k, first, kTile);
   else adamw_tile<P, G, C, kEight, kStream, false>(launch, k, first, (uint32_t)left);
 }
@@ -382,7 +388,7 @@ int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, 
     const auto with_param = [&](auto p, auto c) {
       using P = decltype(p);
       using G = decltype(g);
-      using C = decltype(c);
+      using C = std::remove_pointer_t<decltype(c)>;
       hipStream_t s = (hipStream_t)stream;
       const uint32_t threads = adamw_shape(state_bits == 8).threads;
       if (state_bits == 8 && stream_past_caches) adamw_kernel<P, G, C, true, true><<<launch.n_tiles, threads, 0, s>>>(launch);
@@ -391,8 +397,9 @@ int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, 
       else adamw_kernel<P, G, C, false, false><<<launch.n_tiles, threads, 0, s>>>(launch);
       return (int)hipGetLastError();
     };
-    if (param == ODC_OPS_BF16) return with_param(bf16(), bf16());
-    return copy == ODC_OPS_F16 ? with_param(float(), f16()) : with_param(float(), bf16());
+    if (param == ODC_OPS_BF16) return with_param(bf16(), (void*)nullptr);
+    if (copy == ODC_OPS_NONE) return with_param(float(), (void*)nullptr);
+    return copy == ODC_OPS_F16 ? with_param(float(), (f16*)nullptr) : with_param(float(), (bf16*)nullptr);
   });
 }
 

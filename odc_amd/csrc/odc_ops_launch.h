@@ -115,7 +115,7 @@ struct AdamwLaunch {
   uint32_t first_tile[kAdamwWords / 5 + 1];
   uint64_t words[kAdamwWords];
 
-  static uint32_t words_of(bool eight, bool copies) { return 5 + copies + 2 * eight; }
+  static constexpr uint32_t words_of(bool eight, bool copies) { return 5 + copies + 2 * eight; }
   void set(uint32_t k, const odc_adamw_item& item) {
     uint64_t* w = words + k * words_per_item;
     const void* const pointers[] = {item.param, item.grad, item.exp_avg, item.exp_avg_sq};
