@@ -31,33 +31,24 @@ __device__ __forceinline__ float other_lane(float x) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kControl, 0xf, 0xf, true));
 }
 
-// Combines the values of kLanes neighbouring lanes (a power of two up to 64), in every lane: by data-parallel
-// primitives within 16 lanes and by swaps of rows above, a few cycles each, where a shuffle through LDS takes over 50.
-// Neighbours, pairs, ... : the order is the same for all lanes.
-template <int kLanes, class Op>
-__device__ __forceinline__ float combine_lanes(float x, Op op) {
-  if constexpr (kLanes > 1) x = op(x, other_lane<0xB1>(x));   // quad_perm 1 0 3 2
-  if constexpr (kLanes > 2) x = op(x, other_lane<0x4E>(x));   // quad_perm 2 3 0 1
-  if constexpr (kLanes > 4) x = op(x, other_lane<0x141>(x));  // mirrored within 8
-  if constexpr (kLanes > 8) x = op(x, other_lane<0x140>(x));  // mirrored within 16
+// The sum over kLanes neighbouring lanes (a power of two up to 64), in every lane: by data-parallel primitives within 16
+// lanes and by swaps of rows above, a few cycles each, where a shuffle through LDS takes over 50. Neighbours, pairs,
+// ...: the order is the same for all lanes.
+template <int kLanes>
+__device__ __forceinline__ float sum_lanes(float x) {
+  if constexpr (kLanes > 1) x += other_lane<0xB1>(x);   // quad_perm 1 0 3 2
+  if constexpr (kLanes > 2) x += other_lane<0x4E>(x);   // quad_perm 2 3 0 1
+  if constexpr (kLanes > 4) x += other_lane<0x141>(x);  // mirrored within 8
+  if constexpr (kLanes > 8) x += other_lane<0x140>(x);  // mirrored within 16
   if constexpr (kLanes > 16) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
   if constexpr (kLanes > 32) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
   return x;
-}
-
-template <int kLanes>
-__device__ __forceinline__ float sum_lanes(float x) {
-  return combine_lanes<kLanes>(x, [](float a, float b) { return a + b; });
-}
-template <int kLanes>
-__device__ __forceinline__ float max_lanes(float x) {
-  return combine_lanes<kLanes>(x, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // The sum over the lanes of a wavefront, in every lane.
