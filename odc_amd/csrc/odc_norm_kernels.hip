@@ -343,19 +343,25 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_nor
     }
     __syncthreads();
   }
-  if (threadIdx.x < (uint32_t)kLanes) {
-    float* out = static_cast<float*>(c.workspace) + (uint64_t)blockIdx.x * 2 * width;
+  if (threadIdx.x >= (uint32_t)kLanes) return;
+  const bool alone = gridDim.x == 1;  // nothing to add, and no second launch
+  W* const weight_out = static_cast<W*>(c.grad_weight);
+  W* const bias_out = static_cast<W*>(c.grad_bias);
+  float* const out = static_cast<float*>(c.workspace) + (uint64_t)blockIdx.x * 2 * width;
 #pragma unroll
-    for (int k = 0; k < kVectors; ++k)
+  for (int k = 0; k < kVectors; ++k)
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) {
-        const uint32_t i = (k * kLanes + lane) * kElems + e;
-        if (i < width) {
-          out[i] = dw[k][e];
-          out[width + i] = db[k][e];
-        }
+    for (int e = 0; e < kElems; ++e) {
+      const uint32_t i = (k * kLanes + lane) * kElems + e;
+      if (i >= width) continue;
+      if (!alone) {
+        out[i] = dw[k][e];
+        out[width + i] = db[k][e];
+      } else {
+        if (weight_out) weight_out[i] = from_float<W>(dw[k][e]);
+        if (bias_out) bias_out[i] = from_float<W>(db[k][e]);
       }
-  }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -580,7 +586,7 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
       const uint32_t tiles = (uint32_t)((call.width + kColumnTile - 1) / kColumnTile);
       if (sums) norm_backward_columns_kernel<T><<<dim3(tiles, plan.groups), kWideThreads, 0, s>>>(call, plan.rows_per_group);
     }
-    if (sums) {
+    if (sums && !plan.one_launch()) {
       const uint32_t blocks = (uint32_t)((2 * call.width + kGroupColumns - 1) / kGroupColumns);
       norm_backward_groups_kernel<W><<<blocks, 256, 0, s>>>(call, plan.groups);
     }

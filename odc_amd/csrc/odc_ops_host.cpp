@@ -107,7 +107,8 @@ NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
   plan.shape = dtype == ODC_OPS_F32 ? shape_of(kBackwardShapes32, width, dtype) : shape_of(kBackwardShapes16, width, dtype);
   plan.row_blocks = (uint32_t)std::min<uint64_t>(rows, 8 * kCus);
   if (plan.shape.lanes) {
-    plan.groups = (uint32_t)std::min(ceil_div(rows, kBackwardThreads / plan.shape.lanes), kCus);
+    const uint64_t rounds = ceil_div(rows, kBackwardThreads / plan.shape.lanes);
+    plan.groups = rows && rounds <= kRoundsAlone ? 1 : (uint32_t)std::min(rounds, kCus);
     plan.rows_per_group = 0;
   } else {
     plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kCus));
@@ -173,7 +174,8 @@ int odc_layer_norm(const odc_norm_forward* call, void* stream) {
 
 uint64_t odc_layer_norm_backward_workspace(uint64_t rows, uint64_t width, int32_t dtype) {
   if (check_norm(rows, width, dtype, ODC_OPS_F32) != ODC_OPS_OK || !rows || !width) return 0;
-  return (uint64_t)backward_plan(rows, width, dtype).groups * 2 * width * sizeof(float);
+  const NormBackwardPlan plan = backward_plan(rows, width, dtype);
+  return plan.one_launch() ? 0 : (uint64_t)plan.groups * 2 * width * sizeof(float);
 }
 
 int odc_layer_norm_backward(const odc_norm_backward* call, void* stream) {

@@ -60,7 +60,12 @@ struct NormBackwardPlan {
   uint32_t groups;
   uint32_t row_blocks;      // wide rows: workgroups of the pass over rows
   uint64_t rows_per_group;  // wide rows: of the pass over columns
+
+  // One workgroup alone has nothing to add.
+  bool one_launch() const { return shape.lanes && groups == 1; }
 };
+// A few rows have one workgroup: up to four rounds of them take less than a launch and the workspace do.
+constexpr uint32_t kRoundsAlone = 4;
 constexpr uint32_t kColumnTile = 64;    // columns of one workgroup of the pass over columns
 constexpr uint32_t kGroupColumns = 32;  // and of the one over groups
 

@@ -408,7 +408,7 @@ def train(net, opt, steps, max_norm=None, seed=1):
         if max_norm is not None:
             torch.nn.utils.clip_grad_norm_(net.parameters(), max_norm)
         opt.step()
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
     return losses
 
 
