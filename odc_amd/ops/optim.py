@@ -132,37 +132,40 @@ class AdamW(torch.optim.Optimizer):
         calls, sharded = {}, []
         for number, group in enumerate(self.param_groups):
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                param, grad = _local(p), _local(p.grad)
+                param, grad = _local(p), _local(grad)
                 if param is not p:
                     sharded.append(p)
-                if grad.is_sparse:
+                if grad.layout is not torch.strided:
                     raise TypeError("AdamW: sparse gradients are not supported")
                 if not param.numel():
                     continue
-                if grad.stride() != param.stride() and not (grad.is_contiguous() and param.is_contiguous()):
+                if not (grad.is_contiguous() and param.is_contiguous()) and grad.stride() != param.stride():
                     grad = torch.empty_like(param, dtype=grad.dtype).copy_(grad)
-                steps = self.state[p]["step"] if self.state[p] else 0
-                calls.setdefault((number, steps + 1, param.device, param.dtype, grad.dtype), []).append((p, param, grad))
+                state = self.state[p]
+                key = (number, state["step"] + 1 if state else 1, param.device, param.dtype, grad.dtype)
+                call = calls.get(key)
+                if call is None:
+                    call = calls[key] = ([], [], [], [])
+                for place, value in zip(call, (p, param, grad, state)):
+                    place.append(value)
         if squared_norm is None and self.max_norm is not None and calls:
             if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
-            squared_norm = _host_squared_norm([grad for call in calls.values() for _, _, grad in call])
-        for place, ((number, step, device, _, _), call) in enumerate(calls.items()):
+            squared_norm = _host_squared_norm([grad for _, _, grads, _ in calls.values() for grad in grads])
+        for place, ((number, step, device, _, _), (owners, params, grads, states)) in enumerate(calls.items()):
             group = self.param_groups[number]
             numbers = dict(step=step, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
                            weight_decay=group["weight_decay"], grad_scale=grad_scale, max_norm=self.max_norm,
                            squared_norm=None if squared_norm is None else squared_norm.to(device))
             # another seed for every step, and for every call of a step
             seed = (self.seed * 0x9E3779B1 + step * 0x85EB + place * 0x27D4EB2F) & 0xFFFFFFFF
-            states = []
-            for p, param, _ in call:
-                state = self.state[p]
-                if not state:
-                    self._begin(state, p, param)
-                states.append(state)
-            _, params, grads = zip(*call)
+            if step == 1:
+                for p, param, state in zip(owners, params, states):
+                    if not state:
+                        self._begin(state, p, param)
             if self.state_bits == 8:
                 adamw_step_8bit(params, grads, *([s[name] for s in states] for name in _STATES_8BIT), seed=seed, **numbers)
             else:
@@ -201,9 +204,10 @@ class AdamW(torch.optim.Optimizer):
 
 
 _STATES_8BIT = ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")
+_PLAIN = (Tensor, torch.nn.Parameter)
 _host_squared_norm = squared_norm
 
 
 def _local(t: Tensor) -> Tensor:
     """The memory behind a parameter, a gradient or a state: of a DTensor its shard here."""
-    return getattr(t, "_local_tensor", t)
+    return t if type(t) in _PLAIN else getattr(t, "_local_tensor", t)
