@@ -66,8 +66,7 @@ struct NormBackwardPlan {
 };
 // A few rows have one workgroup: up to four rounds of them take less than a launch and the workspace do.
 constexpr uint32_t kRoundsAlone = 4;
-constexpr uint32_t kColumnTile = 64;    // columns of one workgroup of the pass over columns
-constexpr uint32_t kGroupColumns = 32;  // and of the one over groups
+constexpr uint32_t kGroupColumns = 32;  // columns of one workgroup of the pass over groups
 
 // ---- lists of tensors -----------------------------------------------------------------------------
 // A dispatch counts its work-items in 32 bits.
