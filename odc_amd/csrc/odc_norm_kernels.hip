@@ -129,7 +129,7 @@ __device__ __forceinline__ void row_sums(float (&x)[kValues], float* scratch) {
 
 // A row is read once and stays in the registers of its lanes: mean, then the variance about it (not the difference of two large
 // sums), then the output. Weights stay in registers for all rows of a workgroup; the next row is on its way meanwhile: 64 KiB in
-// flight on a CU. 16384 x 4096 bf16 44 us (6.1 TB/s), 4096 x 4096 13.4 (half of it from the last-level cache's side of HBM),
+// flight on a CU. 16384 x 4096 bf16 44 us (6.1 TB/s), 4096 x 4096 13.4 (5.0),
 // 16384 x 14336 with a residual 323 (5.8 TB/s), 2048 x 256 fp32 3.0.
 template <class T, class W, int kLanes, int kVectors, RowAccess kAccess, bool kAdd>
 __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads) void norm_forward_kernel(odc_norm_forward c) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
 // grad_input and keeps the sums for weight and bias of its lanes' columns in registers; at the end the rows that it had
 // at once are added in LDS, upper half onto lower half, and go to its row of the workspace.
 // 16384 x 4096 bf16 74 us (5.4 TB/s), 4096 x 4096 25 (4.0: 16 rows to a workgroup, start and end are a third of it), 16384 x
-// 14336 with a residual 326 (5.8). In three passes through the caches, without the rows in registers: 1.4 ms of 2.6 for the last.
+// 14336 with a residual 326 (5.8).
 template <class T, class W, int kLanes, int kVectors, RowAccess kAccess>
 __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(odc_norm_backward c) {
   constexpr int kThreads = kBackwardThreads, kElems = Vector<T>::kElems, kRows = kThreads / kLanes;
