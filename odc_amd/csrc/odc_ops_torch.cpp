@@ -103,19 +103,23 @@ class WithoutGil {
   PyThreadState* state_;
 };
 
+// The items of a sequence. They are held for as long as this is there: while a call has let go of the GIL, another thread
+// may change the list that they came from.
 class Sequence {
  public:
-  Sequence(PyObject* o, const char* what) : fast_(PySequence_Fast(o, what)) {
-    if (!fast_) throw Failed();
+  Sequence(PyObject* o, const char* what) : items_(PySequence_Check(o) ? PySequence_Tuple(o) : nullptr) {
+    if (items_) return;
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, what);
+    throw Failed();
   }
-  ~Sequence() { Py_DECREF(fast_); }
+  ~Sequence() { Py_DECREF(items_); }
   Sequence(const Sequence&) = delete;
   Sequence& operator=(const Sequence&) = delete;
-  Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast_); }
-  PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast_, i); }
+  Py_ssize_t size() const { return PyTuple_GET_SIZE(items_); }
+  PyObject* operator[](Py_ssize_t i) const { return PyTuple_GET_ITEM(items_, i); }
 
  private:
-  PyObject* fast_;
+  PyObject* items_;
 };
 
 void expect_args(Py_ssize_t n, Py_ssize_t want) {

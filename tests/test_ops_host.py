@@ -64,6 +64,18 @@ def test_tensors_of_the_cpu_are_refused():
         ops.dequantize_blocks(x.to(torch.float8_e4m3fn), x.to(torch.float8_e8m0fnu))
 
 
+def test_what_is_no_list_is_refused():
+    x = torch.randn(4)
+    with pytest.raises(TypeError, match="sequence"):
+        ops.adamw_step(5, [x], [x], [x], step=1, lr=1e-3)
+    with pytest.raises(TypeError):
+        ops.squared_norm(5)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        ops.squared_norm([5])
+    with pytest.raises(ValueError, match="no tensors"):
+        ops.squared_norm(iter([]))
+
+
 def test_optimizer_arguments():
     p = torch.nn.Parameter(torch.ones(3))
     opt = ops.AdamW([p], lr=0.5, betas=(0.8, 0.9), eps=1e-6, weight_decay=0.0, state_bits=8, max_norm=1.0, seed=3)
