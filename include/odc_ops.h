@@ -41,7 +41,7 @@ typedef enum odc_ops_dtype {
 } odc_ops_dtype;
 
 /* -- layer norm -------------------------------------------------------------------------------------
- * Rows of `width` elements; a row's elements are neighbours, rows lie `..._stride` elements apart
+ * Rows of `width` elements (2^26 at most); a row's elements are neighbours, rows lie `..._stride` elements apart
  * (any stride, 0 included, for what is read). What is written is dense: row i at i * width.
  *
  *   total  = input + residual, rounded to `dtype`     (only with a residual; else total = input)

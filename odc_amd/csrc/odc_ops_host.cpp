@@ -39,11 +39,15 @@ bool spans_too_much(uint64_t rows, uint64_t stride, uint64_t width) {
 constexpr uint64_t kLastLevelCache = uint64_t(256) << 20;
 
 // ---- layer norm -----------------------------------------------------------------------------------
+// The pass over groups has 256 threads for 32 of twice as many columns, and a dispatch counts them in 32 bits.
+constexpr uint64_t kMostColumns = uint64_t(1) << 26;
+static_assert(2 * kMostColumns / kGroupColumns <= most_workgroups(256), "too many workgroups");
+
 int check_norm(uint64_t rows, uint64_t width, int32_t dtype, int32_t weight_dtype) {
   if (!is_float_type(dtype) || !is_float_type(weight_dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d or %d", dtype, weight_dtype);
   if (weight_dtype != dtype && weight_dtype != ODC_OPS_F32)
     return fail(ODC_OPS_ERR_UNSUPPORTED, "weights have the dtype of the input or fp32");
-  if (width > 1u << 30) return fail(ODC_OPS_ERR_INVALID, "rows of %llu elements are too long", (unsigned long long)width);
+  if (width > kMostColumns) return fail(ODC_OPS_ERR_INVALID, "rows of %llu elements are too long", (unsigned long long)width);
   if (spans_too_much(rows, width, width)) return fail(ODC_OPS_ERR_INVALID, "sizes overflow: %llu rows of %llu", (unsigned long long)rows, (unsigned long long)width);
   return ODC_OPS_OK;
 }

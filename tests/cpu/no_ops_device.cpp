@@ -105,7 +105,7 @@ void check_layer_norm() {
   refused([](auto& g) { g.dtype = 3; });
   refused([](auto& g) { g.dtype = ODC_OPS_NONE; });
   refused([](auto& g) { g.weight_dtype = ODC_OPS_F16; });
-  refused([](auto& g) { g.width = uint64_t(1) << 31; });
+  refused([](auto& g) { g.width = g.input_stride = (uint64_t(1) << 26) + 1; });
   refused([](auto& g) { g.rows = uint64_t(1) << 58; });
   refused([](auto& g) { g.input_stride = uint64_t(1) << 58; });
   f.rows = 0;
