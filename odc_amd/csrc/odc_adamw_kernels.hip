@@ -375,32 +375,26 @@ int with_type(int32_t dtype, Body body) {
 
 }  // namespace
 
-int launch_squared_norm(int32_t dtype, bool stream_past_caches, const SquaredNormLaunch& launch, uint32_t blocks, double* partials, void* stream) {
+int launch_squared_norm(int32_t dtype, bool stream_past_caches, const SquaredNormLaunch& l, uint32_t blocks, double* partials, void* stream) {
   return with_type(dtype, [&](auto t) {
-    if (stream_past_caches) squared_norm_kernel<decltype(t), true><<<blocks, 256, 0, (hipStream_t)stream>>>(launch, partials);
-    else squared_norm_kernel<decltype(t), false><<<blocks, 256, 0, (hipStream_t)stream>>>(launch, partials);
-    return (int)hipGetLastError();
+    using T = decltype(t);
+    return launch(stream_past_caches ? squared_norm_kernel<T, true> : squared_norm_kernel<T, false>, blocks, 256, stream, l, partials);
   });
 }
 
 int launch_squared_norm_total(const double* partials, uint32_t n, float* result, void* stream) {
-  squared_norm_total_kernel<<<1, 256, 0, (hipStream_t)stream>>>(partials, n, result);
-  return (int)hipGetLastError();
+  return launch(squared_norm_total_kernel, 1, 256, stream, partials, n, result);
 }
 
-int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, bool stream_past_caches, const AdamwLaunch& launch, void* stream) {
+int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, bool stream_past_caches, const AdamwLaunch& l, void* stream) {
   return with_type(grad, [&](auto g) {
     const auto with_param = [&](auto p, auto c) {
       using P = decltype(p);
       using G = decltype(g);
       using C = std::remove_pointer_t<decltype(c)>;
-      hipStream_t s = (hipStream_t)stream;
-      const uint32_t threads = adamw_shape(state_bits == 8).threads;
-      if (state_bits == 8 && stream_past_caches) adamw_kernel<P, G, C, true, true><<<launch.n_tiles, threads, 0, s>>>(launch);
-      else if (state_bits == 8) adamw_kernel<P, G, C, true, false><<<launch.n_tiles, threads, 0, s>>>(launch);
-      else if (stream_past_caches) adamw_kernel<P, G, C, false, true><<<launch.n_tiles, threads, 0, s>>>(launch);
-      else adamw_kernel<P, G, C, false, false><<<launch.n_tiles, threads, 0, s>>>(launch);
-      return (int)hipGetLastError();
+      const auto kernel = state_bits == 8 ? (stream_past_caches ? adamw_kernel<P, G, C, true, true> : adamw_kernel<P, G, C, true, false>)
+                                          : (stream_past_caches ? adamw_kernel<P, G, C, false, true> : adamw_kernel<P, G, C, false, false>);
+      return launch(kernel, l.n_tiles, adamw_shape(state_bits == 8).threads, stream, l);
     };
     if (param == ODC_OPS_BF16) return with_param(bf16(), (void*)nullptr);
     if (copy == ODC_OPS_NONE) return with_param(float(), (void*)nullptr);
@@ -410,10 +404,10 @@ int launch_adamw(int32_t param, int32_t grad, int32_t copy, int32_t state_bits, 
 
 int launch_dequantize(const void* codes, const void* scales, void* values, uint64_t elems, int32_t dtype, void* stream) {
   return with_type(dtype, [&](auto t) {
-    constexpr uint32_t kTile = 256 * Vector<decltype(t)>::kElems;
-    dequantize_kernel<decltype(t)><<<(uint32_t)((elems + kTile - 1) / kTile), 256, 0, (hipStream_t)stream>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<decltype(t)*>(values), elems);
-    return (int)hipGetLastError();
+    using T = decltype(t);
+    constexpr uint32_t kTile = 256 * Vector<T>::kElems;
+    return launch(dequantize_kernel<T>, (uint32_t)((elems + kTile - 1) / kTile), 256, stream, static_cast<const uint8_t*>(codes),
+                  static_cast<const uint8_t*>(scales), static_cast<T*>(values), elems);
   });
 }
 

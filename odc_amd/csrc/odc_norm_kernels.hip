@@ -658,21 +658,19 @@ int launch_norm_forward(const odc_norm_forward& call, const NormForwardPlan& pla
   return with_types(call.dtype, call.weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    hipStream_t s = (hipStream_t)stream;
-    if (!plan.shape.lanes) {
-      norm_forward_wide_kernel<T, W><<<plan.blocks, kWideThreads, 0, s>>>(call);
-    } else {
-      with_shape<kForwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
-        constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
-        constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
-        with_access<kLanes>(plan.access, [&](auto access) {
-          with_truth(call.residual != nullptr, [&](auto add) {
-            norm_forward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value, decltype(add)::value><<<plan.blocks, kThreads, 0, s>>>(call);
-          });
+    if (!plan.shape.lanes) return launch(norm_forward_wide_kernel<T, W>, plan.blocks, kWideThreads, stream, call);
+    int status = (int)hipErrorInvalidDeviceFunction;
+    with_shape<kForwardShapes>(plan.shape, [&](auto lanes, auto vectors) {
+      constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
+      constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
+      with_access<kLanes>(plan.access, [&](auto access) {
+        with_truth(call.residual != nullptr, [&](auto add) {
+          status = launch(norm_forward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value, decltype(add)::value>, plan.blocks, kThreads,
+                          stream, call);
         });
       });
-    }
-    return (int)hipGetLastError();
+    });
+    return status;
   });
 }
 
@@ -680,28 +678,29 @@ int launch_norm_backward(const odc_norm_backward& call, const NormBackwardPlan& 
   return with_types(call.dtype, call.weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    hipStream_t s = (hipStream_t)stream;
     const bool sums = call.grad_weight || call.grad_bias;
+    int status = 0;
     if (plan.shape.lanes && plan.groups) {
-      const auto launch = [&](auto lanes, auto vectors) {
+      status = (int)hipErrorInvalidDeviceFunction;
+      const auto launch_rows = [&](auto lanes, auto vectors) {
         constexpr int kLanes = decltype(lanes)::value, kVectors = decltype(vectors)::value;
         with_access<kLanes>(plan.access, [&](auto access) {
-          norm_backward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value><<<plan.groups, kBackwardThreads, 0, s>>>(call);
+          status = launch(norm_backward_kernel<T, W, kLanes, kVectors, (RowAccess)decltype(access)::value>, plan.groups, kBackwardThreads, stream, call);
         });
       };
-      if constexpr (sizeof(T) == 4) with_shape<kBackwardShapes32>(plan.shape, launch);
-      else with_shape<kBackwardShapes16>(plan.shape, launch);
+      if constexpr (sizeof(T) == 4) with_shape<kBackwardShapes32>(plan.shape, launch_rows);
+      else with_shape<kBackwardShapes16>(plan.shape, launch_rows);
     } else if (plan.groups) {
-      if (call.grad_input) norm_backward_rows_kernel<T, W><<<plan.row_blocks, kWideThreads, 0, s>>>(call);
+      if (call.grad_input) status = launch(norm_backward_rows_kernel<T, W>, plan.row_blocks, kWideThreads, stream, call);
       constexpr uint32_t kColumns = 64 * Vector<T>::kElems;
       const uint32_t tiles = (uint32_t)((call.width + kColumns - 1) / kColumns);
-      if (sums) norm_backward_columns_kernel<T><<<dim3(tiles, plan.groups), kWideThreads, 0, s>>>(call, plan.rows_per_group);
+      if (!status && sums) status = launch(norm_backward_columns_kernel<T>, dim3(tiles, plan.groups), kWideThreads, stream, call, plan.rows_per_group);
     }
-    if (sums && !plan.one_launch()) {
+    if (!status && sums && !plan.one_launch()) {
       const uint32_t blocks = (uint32_t)((2 * call.width + kGroupColumns - 1) / kGroupColumns);
-      norm_backward_groups_kernel<W><<<blocks, 256, 0, s>>>(call, plan.groups);
+      status = launch(norm_backward_groups_kernel<W>, blocks, 256, stream, call, plan.groups);
     }
-    return (int)hipGetLastError();
+    return status;
   });
 }
 

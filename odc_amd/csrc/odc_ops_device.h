@@ -13,6 +13,16 @@ namespace odc_ops_device {
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
+// `kernel` with what it takes; returns the launch's own status. (hipGetLastError() would also report what an earlier,
+// unrelated HIP call of the same host thread left behind, and make a launch that runs look failed.)
+template <class T>
+struct Same { typedef T type; };
+template <class... P>
+int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, void* stream, const typename Same<P>::type&... values) {
+  void* args[] = {const_cast<void*>(static_cast<const void*>(&values))...};
+  return (int)hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), args, 0, static_cast<hipStream_t>(stream));
+}
+
 template <class T>
 __device__ __forceinline__ float to_float(T x) { return (float)x; }
 template <class T>
