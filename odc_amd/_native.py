@@ -70,6 +70,7 @@ OPS_EXPORTED_SYMBOLS = (
     "odc_squared_norm",
     "odc_squared_norm_workspace",
     "odc_adamw",
+    "odc_adamw_check",
     "odc_dequantize_blocks",
     "odc_ops_last_error",
     "odc_ops_abi_version",

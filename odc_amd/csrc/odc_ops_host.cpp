@@ -247,7 +247,7 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
   return launched(odc_ops_device::launch_squared_norm_total(partials, done, result, stream));
 }
 
-int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_numbers* numbers, void* stream) {
+int odc_adamw_check(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_numbers* numbers) {
   if (!numbers) return fail(ODC_OPS_ERR_INVALID, "numbers is NULL");
   if (!items && n_items) return fail(ODC_OPS_ERR_INVALID, "items is NULL");
   const odc_adamw_numbers& a = *numbers;
@@ -275,6 +275,13 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
         (a.state_bits == 32 && (!aligned(it.exp_avg, 4) || !aligned(it.exp_avg_sq, 4))))
       return fail(ODC_OPS_ERR_INVALID, "item %u: a pointer is not aligned to its element", i);
   }
+  return ODC_OPS_OK;
+}
+
+int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_numbers* numbers, void* stream) {
+  ODC_OPS_TRY(odc_adamw_check(items, n_items, numbers));
+  const odc_adamw_numbers& a = *numbers;
+  const AdamwShape shape = adamw_shape(a.state_bits == 8);
   const uint32_t bytes = 2 * bytes_of(a.param_dtype) + bytes_of(a.grad_dtype) + (a.state_bits == 32 ? 16 : 4);
   const bool past_caches = all_elems(items, n_items) > kLastLevelCache / bytes;
   const double t = (double)a.step;

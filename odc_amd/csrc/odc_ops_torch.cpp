@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <memory>
 #include <optional>
 #include <string>
 #include <utility>
@@ -38,6 +39,7 @@ decltype(&odc_layer_norm_backward_workspace) p_layer_norm_backward_workspace = n
 decltype(&odc_squared_norm) p_squared_norm = nullptr;
 decltype(&odc_squared_norm_workspace) p_squared_norm_workspace = nullptr;
 decltype(&odc_adamw) p_adamw = nullptr;
+decltype(&odc_adamw_check) p_adamw_check = nullptr;
 decltype(&odc_dequantize_blocks) p_dequantize_blocks = nullptr;
 decltype(&odc_ops_last_error) p_ops_last_error = nullptr;
 
@@ -55,6 +57,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     ODC_BIND(squared_norm)
     ODC_BIND(squared_norm_workspace)
     ODC_BIND(adamw)
+    ODC_BIND(adamw_check)
     ODC_BIND(dequantize_blocks)
     ODC_BIND(ops_last_error)
 #undef ODC_BIND
@@ -62,7 +65,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   if (!p_layer_norm || !p_layer_norm_backward || !p_layer_norm_backward_workspace || !p_squared_norm ||
-      !p_squared_norm_workspace || !p_adamw || !p_dequantize_blocks || !p_ops_last_error) {
+      !p_squared_norm_workspace || !p_adamw || !p_adamw_check || !p_dequantize_blocks || !p_ops_last_error) {
     PyErr_SetString(PyExc_RuntimeError, "bind: an entry point is missing");
     return nullptr;
   }
@@ -568,47 +571,51 @@ class Beside {
 
 constexpr int64_t kBlock = 32;
 
-// adamw(params, grads, exp_avgs, exp_avg_scales or None, exp_avg_sqs or roots, their scales or None, copies or None,
-//       squared_norm or None, step, lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm, seed or None)
-PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded([&]() -> PyObject* {
-    expect_args(n, 17);
-    const Sequence params(args[0], "params are a sequence");
-    const Py_ssize_t count = params.size();
-    Beside grads(args[1], "grads", count), m(args[2], "exp_avgs", count), m_scale(args[3], "exp_avg_scales", count);
-    Beside v(args[4], args[3] == Py_None ? "exp_avg_sqs" : "exp_avg_roots", count), v_scale(args[5], "exp_avg_root_scales", count);
-    Beside copies(args[6], "copies", count);
-    const at::Tensor squared_norm = as_optional_tensor(args[7], "squared_norm");
-    const bool eight = m_scale.given();
-    odc_adamw_numbers numbers = {};
+// A call of odc_adamw: its tensors, held and checked, and the structures that name them.
+class AdamwCall {
+ public:
+  // params, grads, exp_avgs, exp_avg_scales or None, exp_avg_sqs or roots, their scales or None, copies or None,
+  // squared_norm or None, step, lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm, seed or None
+  static constexpr Py_ssize_t kArguments = 17;
+
+  explicit AdamwCall(PyObject* const* args)
+      : params_(args[0], "params are a sequence"),
+        count_(params_.size()),
+        grads_(args[1], "grads", count_),
+        m_(args[2], "exp_avgs", count_),
+        m_scale_(args[3], "exp_avg_scales", count_),
+        v_(args[4], args[3] == Py_None ? "exp_avg_sqs" : "exp_avg_roots", count_),
+        v_scale_(args[5], "exp_avg_root_scales", count_),
+        copies_(args[6], "copies", count_),
+        squared_norm_(as_optional_tensor(args[7], "squared_norm")) {
+    const bool eight = m_scale_.given();
     const int64_t step = as_int(args[8]);
     if (step < 1) raise(PyExc_ValueError, "the first step is 1");
-    numbers.step = (uint64_t)step;
-    numbers.lr = as_double(args[9]);
-    numbers.beta1 = as_double(args[10]);
-    numbers.beta2 = as_double(args[11]);
-    numbers.eps = as_double(args[12]);
-    numbers.weight_decay = as_double(args[13]);
-    numbers.grad_scale = as_double(args[14]);
-    numbers.max_norm = as_double(args[15]);
+    numbers_.step = (uint64_t)step;
+    numbers_.lr = as_double(args[9]);
+    numbers_.beta1 = as_double(args[10]);
+    numbers_.beta2 = as_double(args[11]);
+    numbers_.eps = as_double(args[12]);
+    numbers_.weight_decay = as_double(args[13]);
+    numbers_.grad_scale = as_double(args[14]);
+    numbers_.max_norm = as_double(args[15]);
     if (args[16] != Py_None) {
       PyObject* masked = PyNumber_Index(args[16]);
       if (!masked) throw Failed();
-      numbers.seed = (uint32_t)PyLong_AsUnsignedLongLongMask(masked);  // its low 32 bits
+      numbers_.seed = (uint32_t)PyLong_AsUnsignedLongLongMask(masked);  // its low 32 bits
       Py_DECREF(masked);
-      numbers.stochastic = 1;
+      numbers_.stochastic = 1;
     } else if (eight) {
       raise(PyExc_ValueError, "states in 8 bits are rounded by random numbers: give a seed, another one for every step");
     }
-    if (!count) Py_RETURN_NONE;
-    std::vector<odc_adamw_item> items;
+    if (!count_) return;
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    items.reserve((size_t)count);
-    spans.reserve((size_t)count);
-    const at::Tensor& first = as_tensor(params[0], "params");
+    items_.reserve((size_t)count_);
+    spans.reserve((size_t)count_);
+    const at::Tensor& first = as_tensor(params_[0], "params");
     expect_gpu("params", first);
-    for (Py_ssize_t k = 0; k < count; ++k) {
-      const at::Tensor& p = as_tensor(params[k], "params");
+    for (Py_ssize_t k = 0; k < count_; ++k) {
+      const at::Tensor& p = as_tensor(params_[k], "params");
       expect_device("params", p, first.device());
       if (p.scalar_type() != first.scalar_type()) raise(PyExc_TypeError, "params: tensors of one call have one dtype");
       if (!p.is_non_overlapping_and_dense()) raise(PyExc_ValueError, "params: tensor %zd is not dense", k);
@@ -616,40 +623,91 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const int64_t numel = p.numel(), blocks = (numel + kBlock - 1) / kBlock;
       item.elems = (uint64_t)numel;
       item.param = p.data_ptr();
-      item.grad = grads.like(k, p);
-      item.exp_avg = eight ? m.flat(k, p.device(), numel) : m.like(k, p);
-      item.exp_avg_sq = eight ? v.flat(k, p.device(), numel) : v.like(k, p);
-      item.exp_avg_scale = m_scale.flat(k, p.device(), blocks);
-      item.exp_avg_sq_scale = v_scale.flat(k, p.device(), blocks);
-      item.copy = copies.like(k, p);
-      items.push_back(item);
+      item.grad = grads_.like(k, p);
+      item.exp_avg = eight ? m_.flat(k, p.device(), numel) : m_.like(k, p);
+      item.exp_avg_sq = eight ? v_.flat(k, p.device(), numel) : v_.like(k, p);
+      item.exp_avg_scale = m_scale_.flat(k, p.device(), blocks);
+      item.exp_avg_sq_scale = v_scale_.flat(k, p.device(), blocks);
+      item.copy = copies_.like(k, p);
+      items_.push_back(item);
       if (numel) spans.emplace_back((uintptr_t)item.param, (uintptr_t)item.param + (uintptr_t)numel * p.element_size());
     }
     if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());  // (the allocator's order, as a rule)
     for (size_t k = 1; k < spans.size(); ++k)
       if (spans[k].first < spans[k - 1].second) raise(PyExc_ValueError, "params: two tensors overlap");
-    numbers.param_dtype = float_code("params", first);
-    if (numbers.param_dtype == ODC_OPS_F16) raise(PyExc_TypeError, "params: fp32 or bf16 is supported, not Half");
-    numbers.grad_dtype = dtype_code(grads.dtype());
-    if (numbers.grad_dtype == ODC_OPS_NONE) raise(PyExc_TypeError, "grads: bf16, fp16 or fp32 is supported, not %s", at::toString(grads.dtype()));
-    numbers.copy_dtype = copies.given() ? dtype_code(copies.dtype()) : (int32_t)ODC_OPS_NONE;
-    if (copies.given() && (numbers.copy_dtype < 0 || numbers.copy_dtype == ODC_OPS_F32 || numbers.param_dtype != ODC_OPS_F32))
+    numbers_.param_dtype = float_code("params", first);
+    if (numbers_.param_dtype == ODC_OPS_F16) raise(PyExc_TypeError, "params: fp32 or bf16 is supported, not Half");
+    numbers_.grad_dtype = dtype_code(grads_.dtype());
+    if (numbers_.grad_dtype == ODC_OPS_NONE) raise(PyExc_TypeError, "grads: bf16, fp16 or fp32 is supported, not %s", at::toString(grads_.dtype()));
+    numbers_.copy_dtype = copies_.given() ? dtype_code(copies_.dtype()) : (int32_t)ODC_OPS_NONE;
+    if (copies_.given() && (numbers_.copy_dtype < 0 || numbers_.copy_dtype == ODC_OPS_F32 || numbers_.param_dtype != ODC_OPS_F32))
       raise(PyExc_TypeError, "copies: bf16 or fp16, of fp32 parameters");
-    numbers.state_bits = eight ? 8 : 32;
-    for (const Beside* states : {&m, &v}) states->expect(eight ? at::kFloat8_e4m3fn : at::kFloat);
-    for (const Beside* scales : {&m_scale, &v_scale}) scales->expect(at::kFloat8_e8m0fnu);
-    if (squared_norm.defined()) {
-      expect_device("squared_norm", squared_norm, first.device());
-      if (squared_norm.numel() != 1 || squared_norm.scalar_type() != at::kFloat) raise(PyExc_TypeError, "squared_norm: expected one fp32 value");
-      numbers.squared_norm = static_cast<const float*>(squared_norm.data_ptr());
+    numbers_.state_bits = eight ? 8 : 32;
+    for (const Beside* states : {&m_, &v_}) states->expect(eight ? at::kFloat8_e4m3fn : at::kFloat);
+    for (const Beside* scales : {&m_scale_, &v_scale_}) scales->expect(at::kFloat8_e8m0fnu);
+    if (squared_norm_.defined()) {
+      expect_device("squared_norm", squared_norm_, first.device());
+      if (squared_norm_.numel() != 1 || squared_norm_.scalar_type() != at::kFloat) raise(PyExc_TypeError, "squared_norm: expected one fp32 value");
+      numbers_.squared_norm = static_cast<const float*>(squared_norm_.data_ptr());
     }
+  }
+
+  // The checks of the C ABI's side.
+  void check() const {
+    if (count_) check_status(p_adamw_check(items_.data(), (uint32_t)count_, &numbers_));
+  }
+
+  void launch() const {
+    if (!count_) return;
     {
+      const at::Device device = THPVariable_Unpack(params_[0]).device();
       WithoutGil nobody;
-      const c10::DeviceGuard guard(first.device());
-      check_status(p_adamw(items.data(), (uint32_t)count, &numbers, current_stream(first.device())));
+      const c10::DeviceGuard guard(device);
+      check_status(p_adamw(items_.data(), (uint32_t)count_, &numbers_, current_stream(device)));
     }
-    for (Py_ssize_t k = 0; k < count; ++k) mark_written(THPVariable_Unpack(params[k]));
-    for (const Beside* written : {&m, &m_scale, &v, &v_scale, &copies}) written->mark();
+    for (Py_ssize_t k = 0; k < count_; ++k) mark_written(THPVariable_Unpack(params_[k]));
+    for (const Beside* written : {&m_, &m_scale_, &v_, &v_scale_, &copies_}) written->mark();
+  }
+
+ private:
+  Sequence params_;
+  Py_ssize_t count_;
+  Beside grads_, m_, m_scale_, v_, v_scale_, copies_;
+  at::Tensor squared_norm_;
+  odc_adamw_numbers numbers_ = {};
+  std::vector<odc_adamw_item> items_;
+};
+
+// adamw(AdamwCall's arguments)
+PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, AdamwCall::kArguments);
+    AdamwCall(args).launch();
+    Py_RETURN_NONE;
+  });
+}
+
+constexpr const char* kPrepared = "odc_ops_torch.adamw_prepare";
+
+// adamw_prepare(AdamwCall's arguments) -> a call that nothing is wrong with, for adamw_launch
+PyObject* adamw_prepare(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, AdamwCall::kArguments);
+    auto call = std::make_unique<AdamwCall>(args);
+    call->check();
+    PyObject* capsule = PyCapsule_New(call.get(), kPrepared, [](PyObject* c) { delete static_cast<AdamwCall*>(PyCapsule_GetPointer(c, kPrepared)); });
+    if (capsule) (void)call.release();
+    return capsule;
+  });
+}
+
+// adamw_launch(what adamw_prepare returned)
+PyObject* adamw_launch(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 1);
+    const auto* call = static_cast<const AdamwCall*>(PyCapsule_GetPointer(args[0], kPrepared));
+    if (!call) throw Failed();
+    call->launch();
     Py_RETURN_NONE;
   });
 }
@@ -686,6 +744,8 @@ PyMethodDef module_methods[] = {
     ODC_METHOD(layer_norm),
     ODC_METHOD(squared_norm),
     ODC_METHOD(adamw),
+    ODC_METHOD(adamw_prepare),
+    ODC_METHOD(adamw_launch),
     ODC_METHOD(dequantize_blocks),
 #undef ODC_METHOD
     {nullptr, nullptr, 0, nullptr}};

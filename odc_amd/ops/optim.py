@@ -155,27 +155,39 @@ class AdamW(torch.optim.Optimizer):
             if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
             squared_norm = _host_squared_norm([grad for _, _, grads, _ in calls.values() for grad in grads])
-        for place, ((number, step, device, _, _), (owners, params, grads, states)) in enumerate(calls.items()):
-            group = self.param_groups[number]
-            numbers = dict(step=step, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
-                           weight_decay=group["weight_decay"], grad_scale=grad_scale, max_norm=self.max_norm,
-                           squared_norm=None if squared_norm is None else squared_norm.to(device))
-            # another seed for every step, and for every call of a step
-            seed = (self.seed * 0x9E3779B1 + step * 0x85EB + place * 0x27D4EB2F) & 0xFFFFFFFF
-            if step == 1:
-                for p, param, state in zip(owners, params, states):
-                    if not state:
-                        self._begin(state, p, param)
-            if self.state_bits == 8:
-                adamw_step_8bit(params, grads, *([s[name] for s in states] for name in _STATES_8BIT), seed=seed, **numbers)
-            else:
-                adamw_step(params, grads, *([_local(s[name]) for s in states] for name in ("exp_avg", "exp_avg_sq")),
-                           seed=seed if self.stochastic_params else None, **numbers)
-            for state in states:
-                state["step"] = step
-        if sharded:
-            torch.autograd.graph.increment_version(sharded)  # of a DTensor: its local tensor has a counter of its own
-        shards_may_have_changed()
+        # Every call is checked before the first is made: a step that is refused has written nothing.
+        prepared, begun = [], []
+        try:
+            for place, ((number, step, device, _, _), (owners, params, grads, states)) in enumerate(calls.items()):
+                group = self.param_groups[number]
+                # another seed for every step, and for every call of a step
+                seed = (self.seed * 0x9E3779B1 + step * 0x85EB + place * 0x27D4EB2F) & 0xFFFFFFFF
+                if step == 1:
+                    for p, param, state in zip(owners, params, states):
+                        if not state:
+                            begun.append(state)
+                            self._begin(state, p, param)
+                if self.state_bits == 8:
+                    lists = [[s[name] for s in states] for name in _STATES_8BIT]
+                else:
+                    exp_avgs, exp_avg_sqs = ([_local(s[name]) for s in states] for name in ("exp_avg", "exp_avg_sq"))
+                    lists, seed = (exp_avgs, None, exp_avg_sqs, None), seed if self.stochastic_params else None
+                prepared.append((step, states, _host_path.adamw_prepare(
+                    params, grads, *lists, None, None if squared_norm is None else squared_norm.to(device), step, float(group["lr"]),
+                    *group["betas"], group["eps"], group["weight_decay"], grad_scale, 0.0 if self.max_norm is None else self.max_norm, seed)))
+        except BaseException:
+            for state in begun:
+                state.clear()
+            raise
+        try:
+            for step, states, call in prepared:
+                _host_path.adamw_launch(call)
+                for state in states:
+                    state["step"] = step
+        finally:  # (a launch that fails leaves the ones in front of it done)
+            if sharded:
+                torch.autograd.graph.increment_version(sharded)  # of a DTensor: its local tensor has a counter of its own
+            shards_may_have_changed()
         return loss
 
     def _begin(self, state, p, param):
