@@ -20,6 +20,7 @@ bits, another seed for every step. A ``v`` that is not zero is never stored as z
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -86,8 +87,9 @@ def _norm(squared_norm, max_norm):
 
 def dequantize_blocks(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.float32) -> Tensor:
     """What a state in 8 bits stands for: ``codes * scales``, 32 neighbouring codes to a scale. Exact in bf16 and fp32
-    (4 significant bits times a power of two)."""
-    return _host_path.dequantize_blocks(codes, scales, dtype)
+    (4 significant bits times a power of two). Of a sharded parameter's states: what this rank has of them, as long as the
+    largest shard needs (zeros behind its own)."""
+    return _host_path.dequantize_blocks(_local(codes), _local(scales), dtype)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -97,6 +99,10 @@ class AdamW(torch.optim.Optimizer):
     scales; 2.06 bytes per element instead of 8). ``max_norm`` clips the gradients by their norm over all parameters of
     the optimizer; where these are shards, give ``step`` the ``squared_norm`` summed over the ranks. ``seed`` sets
     the random roundings: of states in 8 bits, and of parameters in bf16 beside those or with ``stochastic_params``.
+
+    States of a sharded parameter (a DTensor) are DTensors, so that torch's distributed checkpoint saves every rank's. In
+    8 bits they are blocks of one shard's memory: one row for each shard, as long as the largest needs. They are read again for the
+    same sharding; for another one their shapes do not match, and loading them raises.
 
     ``step`` may not be captured into a HIP graph: the step's number would be a constant of it."""
 
@@ -169,6 +175,8 @@ class AdamW(torch.optim.Optimizer):
                             self._begin(state, p, param)
                 if self.state_bits == 8:
                     lists = [[s[name] for s in states] for name in _STATES_8BIT]
+                    if sharded:
+                        lists = [[_first(t, param.numel(), per) for t, param in zip(one, params)] for one, per in zip(lists, (1, BLOCK) * 2)]
                 else:
                     exp_avgs, exp_avg_sqs = ([_local(s[name]) for s in states] for name in ("exp_avg", "exp_avg_sq"))
                     lists, seed = (exp_avgs, None, exp_avg_sqs, None), seed if self.stochastic_params else None
@@ -196,9 +204,13 @@ class AdamW(torch.optim.Optimizer):
             state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             return
-        n, blocks = param.numel(), -(-param.numel() // BLOCK)
-        for name, size, dtype in zip(_STATES_8BIT, (n, blocks) * 2, (torch.float8_e4m3fn, torch.float8_e8m0fnu) * 2):
-            state[name] = torch.zeros(size, dtype=torch.uint8, device=param.device).view(dtype)
+        n, dtypes = param.numel(), (torch.float8_e4m3fn, torch.float8_e8m0fnu) * 2
+        shards = None
+        if hasattr(p, "placements"):
+            n, shards = _shards_of(p, n)
+        for name, size, dtype in zip(_STATES_8BIT, (n, -(-n // BLOCK)) * 2, dtypes):
+            value = torch.zeros(size, dtype=torch.uint8, device=param.device).view(dtype)
+            state[name] = value if shards is None else _one_of(value, p, shards)
 
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``, which takes every state for one of its parameter's dtype:
@@ -218,6 +230,34 @@ class AdamW(torch.optim.Optimizer):
 _STATES_8BIT = ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")
 _PLAIN = (Tensor, torch.nn.Parameter)
 _host_squared_norm = squared_norm
+
+
+def _shards_of(p, n: int) -> Tuple[int, Tuple[int, ...]]:
+    """Elements of the largest shard of a DTensor (``n`` of them are here), and into how many it is split along each of
+    its dimensions."""
+    longest, shards = list(p.shape), [1] * p.dim()
+    for k, placement in enumerate(p.placements):
+        dim = getattr(placement, "dim", None)
+        if dim is not None:
+            longest[dim], shards[dim] = -(-longest[dim] // p.device_mesh.size(k)), shards[dim] * p.device_mesh.size(k)
+    return max(n, math.prod(longest)), tuple(shards)
+
+
+def _one_of(value: Tensor, p, shards: Tuple[int, ...]) -> Tensor:
+    """``value`` as the part of this rank of a DTensor that is placed as ``p`` is: one row for each of the shards."""
+    from torch.distributed.tensor import DTensor
+
+    shape = (*shards, value.numel())
+    stride = [math.prod(shape[k + 1:]) for k in range(len(shape))]
+    return DTensor.from_local(value.view(*(1 for _ in shards), -1), p.device_mesh, p.placements, run_check=False, shape=torch.Size(shape),
+                              stride=tuple(stride))
+
+
+def _first(state: Tensor, elems: int, per: int) -> Tensor:
+    """Of a state (of a DTensor: its part here, which is as long as the largest shard needs) what belongs to ``elems``
+    elements."""
+    local, n = _local(state), -(-elems // per)
+    return local if local is state or local.numel() == n else local.view(-1)[:n]
 
 
 def _local(t: Tensor) -> Tensor:
