@@ -158,9 +158,12 @@ class AdamW(torch.optim.Optimizer):
                 for place, value in zip(call, (p, param, grad, state)):
                     place.append(value)
         if squared_norm is None and self.max_norm is not None and calls:
-            if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")):
+            grads = [grad for _, _, grads, _ in calls.values() for grad in grads]
+            # The norm of this rank's gradients is not that of all ranks'. (Where they are zero they are zero whatever they are clipped by:
+            # torch's get_optimizer_state_dict begins the states by such a step.)
+            if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")) and any(bool(grad.any()) for grad in grads):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
-            squared_norm = _host_squared_norm([grad for _, _, grads, _ in calls.values() for grad in grads])
+            squared_norm = _host_squared_norm(grads)
         # Every call is checked before the first is made: a step that is refused has written nothing.
         prepared, begun = [], []
         try:

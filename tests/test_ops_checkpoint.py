@@ -133,3 +133,23 @@ def test_every_rank_reads_what_it_wrote(tmp_path, bits, dim):
 
 def test_states_in_8_bits_are_not_read_for_another_sharding(tmp_path):
     on_two_ranks(tmp_path, another_sharding)
+
+
+def own_norm(rank, mesh, path):
+    """A step of torch's own that begins the states has zero gradients, and needs no norm; with others it does, on a rank
+    whose gradients are not zero."""
+    restored(rank, mesh, path, 32, [(8, 32), (101,)], max_norm=1.0)
+    restored(rank, mesh, path + "8", 8, [(8, 32), (101,)], max_norm=1.0)
+    model, opt = fresh(mesh, [(8, 32), (101,)], max_norm=1.0)
+    p, q = model.parameters()
+    p.grad, q.grad = torch.zeros_like(p), torch.zeros_like(q)
+    q.grad._local_tensor[-1] = 1e-30  # its square is no fp32 number
+    with pytest.raises(ValueError, match="shards"):
+        opt.step()
+    q.grad._local_tensor[-1] = float("nan")
+    with pytest.raises(ValueError, match="shards"):
+        opt.step()
+
+
+def test_clipped_shards_are_resumed(tmp_path):
+    on_two_ranks(tmp_path, own_norm)
