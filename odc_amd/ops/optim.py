@@ -135,7 +135,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW.step cannot be captured into a graph: the step's number would be a constant of it")
         if squared_norm is not None and self.max_norm is None:
             raise ValueError("squared_norm without max_norm: there is nothing to clip to")
-        calls, sharded = {}, []
+        calls, sharded, idle = {}, [], []
         for number, group in enumerate(self.param_groups):
             for p in group["params"]:
                 grad = p.grad
@@ -147,6 +147,7 @@ class AdamW(torch.optim.Optimizer):
                 if grad.layout is not torch.strided:
                     raise TypeError("AdamW: sparse gradients are not supported")
                 if not param.numel():
+                    idle.append((p, param))
                     continue
                 if not (grad.is_contiguous() and param.is_contiguous()) and grad.stride() != param.stride():
                     grad = torch.empty_like(param, dtype=grad.dtype).copy_(grad)
@@ -186,6 +187,10 @@ class AdamW(torch.optim.Optimizer):
                 prepared.append((step, states, _host_path.adamw_prepare(
                     params, grads, *lists, None, None if squared_norm is None else squared_norm.to(device), step, float(group["lr"]),
                     *group["betas"], group["eps"], group["weight_decay"], grad_scale, 0.0 if self.max_norm is None else self.max_norm, seed)))
+            for p, param in idle:  # nothing to step, but a shard without elements has states as the other ranks' have
+                if not self.state[p]:
+                    begun.append(self.state[p])
+                    self._begin(self.state[p], p, param)
         except BaseException:
             for state in begun:
                 state.clear()
@@ -195,6 +200,8 @@ class AdamW(torch.optim.Optimizer):
                 _host_path.adamw_launch(call)
                 for state in states:
                     state["step"] = step
+            for p, _ in idle:
+                self.state[p]["step"] += 1
         finally:  # (a launch that fails leaves the ones in front of it done)
             if sharded:
                 torch.autograd.graph.increment_version(sharded)  # of a DTensor: its local tensor has a counter of its own

@@ -153,3 +153,9 @@ def own_norm(rank, mesh, path):
 
 def test_clipped_shards_are_resumed(tmp_path):
     on_two_ranks(tmp_path, own_norm)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_rank_whose_shard_is_empty(tmp_path, bits):
+    """One row over two ranks: the second has nothing of it, and states like the first."""
+    on_two_ranks(tmp_path, restored, bits, [(8, 32), (1, 32)])
