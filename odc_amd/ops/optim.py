@@ -224,7 +224,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``, which takes every state for one of its parameter's dtype:
-        here they keep their own."""
+        here they keep their own. In 32 bits the states of ``torch.optim.AdamW`` are read too (the step's number, a tensor
+        there, becomes an int)."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = set(_STATES_8BIT if self.state_bits == 8 else ("exp_avg", "exp_avg_sq")) | {"step"}
         for state in state_dict["state"].values():
@@ -233,7 +234,9 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
             for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, Tensor):
+                if name == "step":
+                    self.state[p][name] = int(value)
+                elif isinstance(value, Tensor):
                     self.state[p][name] = value.detach().clone().to(p.device)
 
 
