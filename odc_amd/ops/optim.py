@@ -151,7 +151,7 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if not (grad.is_contiguous() and param.is_contiguous()) and grad.stride() != param.stride():
                     grad = torch.empty_like(param, dtype=grad.dtype).copy_(grad)
-                state = self.state[p]
+                state = self.state.get(p) or {}  # (reading self.state[p] would leave an empty one behind)
                 key = (number, state["step"] + 1 if state else 1, param.device, param.dtype, grad.dtype)
                 call = calls.get(key)
                 if call is None:
@@ -175,8 +175,9 @@ class AdamW(torch.optim.Optimizer):
                 if step == 1:
                     for p, param, state in zip(owners, params, states):
                         if not state:
-                            begun.append(state)
+                            begun.append(p)
                             self._begin(state, p, param)
+                            self.state[p] = state
                 if self.state_bits == 8:
                     lists = [[s[name] for s in states] for name in _STATES_8BIT]
                     if sharded:
@@ -188,12 +189,12 @@ class AdamW(torch.optim.Optimizer):
                     params, grads, *lists, None, None if squared_norm is None else squared_norm.to(device), step, float(group["lr"]),
                     *group["betas"], group["eps"], group["weight_decay"], grad_scale, 0.0 if self.max_norm is None else self.max_norm, seed)))
             for p, param in idle:  # nothing to step, but a shard without elements has states as the other ranks' have
-                if not self.state[p]:
-                    begun.append(self.state[p])
+                if not self.state.get(p):
+                    begun.append(p)
                     self._begin(self.state[p], p, param)
         except BaseException:
-            for state in begun:
-                state.clear()
+            for p in begun:
+                self.state.pop(p, None)
             raise
         try:
             for step, states, call in prepared:
@@ -229,7 +230,7 @@ class AdamW(torch.optim.Optimizer):
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = set(_STATES_8BIT if self.state_bits == 8 else ("exp_avg", "exp_avg_sq")) | {"step"}
         for state in state_dict["state"].values():
-            if set(state) != names:
+            if state and set(state) != names:
                 raise ValueError(f"the states are those of another optimizer: {sorted(state)}, not {sorted(names)} (state_bits={self.state_bits})")
         super().load_state_dict(state_dict)
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):

@@ -52,3 +52,36 @@ def test_torchs_states_are_read(calls):
     for p, a, b in zip(ps, m, v):
         assert torch.equal(a, theirs.state[p]["exp_avg"]) and torch.equal(b, theirs.state[p]["exp_avg_sq"])
         assert type(ours.state[p]["step"]) is int and ours.state[p]["step"] == 6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_step_leaves_no_states(calls, bits):
+    ps = parameters(2) + parameters(1, torch.float64)
+    opt = optim.AdamW(ps, state_bits=bits)
+    with pytest.raises(TypeError):
+        opt.step()
+    assert not calls and len(opt.state) == 0 and opt.state_dict()["state"] == {}
+    ps[2].grad = None
+    opt.step()
+    assert len(opt.state) == 2
+    again = optim.AdamW(ps, state_bits=bits)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert again.state[ps[0]]["step"] == again.state[ps[1]]["step"] == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_was_only_looked_at(calls, bits):
+    """``opt.state`` makes an empty state for who asks; it is saved, and no state to the optimizer that reads it."""
+    ps = parameters()
+    opt = optim.AdamW(ps, state_bits=bits)
+    opt.step()
+    ps.append(torch.nn.Parameter(torch.ones(9)))
+    opt.add_param_group({"params": ps[3:]})
+    assert opt.state[ps[3]] == {}
+    saved = copy.deepcopy(opt.state_dict())
+    assert {} in saved["state"].values()
+    again = optim.AdamW([{"params": ps[:3]}, {"params": ps[3:]}], state_bits=bits)
+    again.load_state_dict(saved)
+    ps[3].grad = torch.ones(9)
+    again.step()
+    assert [again.state[p]["step"] for p in ps] == [2, 2, 2, 1]
