@@ -226,12 +226,17 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``, which takes every state for one of its parameter's dtype:
         here they keep their own. In 32 bits the states of ``torch.optim.AdamW`` are read too (the step's number, a tensor
-        there, becomes an int)."""
+        there, becomes an int); options of its that change the step, and that this one does not have, are refused."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = set(_STATES_8BIT if self.state_bits == 8 else ("exp_avg", "exp_avg_sq")) | {"step"}
         for state in state_dict["state"].values():
             if state and set(state) != names:
                 raise ValueError(f"the states are those of another optimizer: {sorted(state)}, not {sorted(names)} (state_bits={self.state_bits})")
+        for group in state_dict["param_groups"]:
+            coupled = group.get("weight_decay") and group.get("decoupled_weight_decay") is False  # torch.optim.Adam's
+            for name, wrong in (("amsgrad", group.get("amsgrad")), ("maximize", group.get("maximize")), ("decoupled_weight_decay=False", coupled)):
+                if wrong:
+                    raise ValueError(f"the states are those of another optimizer: {name} is not supported")
         super().load_state_dict(state_dict)
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
             for name, value in state_dict["state"].get(i, {}).items():

@@ -85,3 +85,24 @@ def test_a_state_that_was_only_looked_at(calls, bits):
     ps[3].grad = torch.ones(9)
     again.step()
     assert [again.state[p]["step"] for p in ps] == [2, 2, 2, 1]
+
+
+@pytest.mark.parametrize("kind,option", [("AdamW", dict(maximize=True)), ("AdamW", dict(amsgrad=True)), ("Adam", dict(weight_decay=0.1)),
+                                         ("Adam", dict(maximize=True))])
+def test_options_that_change_the_step_are_refused(calls, kind, option):
+    """They came with the parameter groups, and were ignored."""
+    ps = parameters()
+    theirs = getattr(torch.optim, kind)(ps, **option)
+    theirs.step()
+    with pytest.raises(ValueError, match="another optimizer"):
+        optim.AdamW(ps).load_state_dict(theirs.state_dict())
+
+
+def test_adam_without_decay_is_read(calls):
+    ps = parameters()
+    theirs = torch.optim.Adam(ps)
+    theirs.step()
+    ours = optim.AdamW(ps)
+    ours.load_state_dict(theirs.state_dict())
+    ours.step()
+    assert calls[0][13] == 0 and calls[0][8] == 2  # no decay, the second step
