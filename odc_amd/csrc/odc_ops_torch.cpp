@@ -7,6 +7,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -172,6 +173,12 @@ void expect_device(const char* what, const at::Tensor& t, const at::Device& devi
   if (t.device() == device) return;
   expect_gpu(what, t);
   if (t.device() != device) raise(PyExc_ValueError, "%s is on %s, not on %s", what, t.device().str().c_str(), device.str().c_str());
+}
+
+// A tangent that the result would not have is one that is taken for zero.
+void expect_no_tangent(const char* what, const at::Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    raise(PyExc_NotImplementedError, "%s: forward-mode derivatives are not supported", what);
 }
 
 void* current_stream(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
@@ -408,6 +415,10 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor input = as_tensor(args[0], "input"), residual = as_optional_tensor(args[1], "residual");
     const at::Tensor weight = as_optional_tensor(args[3], "weight"), bias = as_optional_tensor(args[4], "bias");
     const double eps = as_double(args[5]);
+    expect_no_tangent("input", input);
+    expect_no_tangent("residual", residual);
+    expect_no_tangent("weight", weight);
+    expect_no_tangent("bias", bias);
     std::vector<int64_t> shape;
     if (PyLong_Check(args[2])) {
       shape.push_back(as_int(args[2]));
@@ -479,10 +490,12 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     std::vector<at::Tensor> copies;  // of what is not dense
     items.reserve((size_t)tensors.size());
     const at::Tensor& first = as_tensor(tensors[0], "tensors");
+    expect_no_tangent("tensors", first);
     expect_gpu("tensors", first);
     const int32_t code = float_code("tensors", first);
     for (Py_ssize_t k = 0; k < tensors.size(); ++k) {
       const at::Tensor& t = as_tensor(tensors[k], "tensors");
+      expect_no_tangent("tensors", t);
       expect_device("tensors", t, first.device());
       if (float_code("tensors", t) != code) Py_RETURN_NONE;
       if (t.is_non_overlapping_and_dense()) {
