@@ -5,10 +5,12 @@
 // libodc_ops.so are bound by address (bind()). The GIL is released around allocations and library calls.
 #include <Python.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -173,6 +175,13 @@ void expect_device(const char* what, const at::Tensor& t, const at::Device& devi
   if (t.device() == device) return;
   expect_gpu(what, t);
   if (t.device() != device) raise(PyExc_ValueError, "%s is on %s, not on %s", what, t.device().str().c_str(), device.str().c_str());
+}
+
+// These calls are no operations to torch's dispatcher. A program that records operations would have recorded the
+// allocation of their results alone.
+void expect_no_tracing(const char* call) {
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    raise(PyExc_NotImplementedError, "%s cannot be traced: it is no operation of torch's", call);
 }
 
 // A tangent that the result would not have is one that is taken for zero.
@@ -412,6 +421,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 6);
+    expect_no_tracing("layer_norm");
     const at::Tensor input = as_tensor(args[0], "input"), residual = as_optional_tensor(args[1], "residual");
     const at::Tensor weight = as_optional_tensor(args[3], "weight"), bias = as_optional_tensor(args[4], "bias");
     const double eps = as_double(args[5]);
@@ -484,6 +494,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 1);
+    expect_no_tracing("squared_norm");
     const Sequence tensors(args[0], "tensors are a sequence");
     if (!tensors.size()) raise(PyExc_ValueError, "the squared norm of no tensors has no device to be on");
     std::vector<odc_span_item> items;
@@ -695,6 +706,7 @@ class AdamwCall {
 PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, AdamwCall::kArguments);
+    expect_no_tracing("adamw_step");
     AdamwCall(args).launch();
     Py_RETURN_NONE;
   });
@@ -706,6 +718,7 @@ constexpr const char* kPrepared = "odc_ops_torch.adamw_prepare";
 PyObject* adamw_prepare(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, AdamwCall::kArguments);
+    expect_no_tracing("adamw_step");
     auto call = std::make_unique<AdamwCall>(args);
     call->check();
     PyObject* capsule = PyCapsule_New(call.get(), kPrepared, [](PyObject* c) { delete static_cast<AdamwCall*>(PyCapsule_GetPointer(c, kPrepared)); });
@@ -729,6 +742,7 @@ PyObject* adamw_launch(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* dequantize_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 3);
+    expect_no_tracing("dequantize_blocks");
     const at::Tensor &codes = as_tensor(args[0], "codes"), &scales = as_tensor(args[1], "scales");
     if (!THPDtype_Check(args[2])) raise(PyExc_TypeError, "expected a torch.dtype, got %s", Py_TYPE(args[2])->tp_name);
     const at::ScalarType type = reinterpret_cast<THPDtype*>(args[2])->scalar_type;
