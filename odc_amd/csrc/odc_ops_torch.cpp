@@ -15,6 +15,8 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -499,6 +501,7 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!tensors.size()) raise(PyExc_ValueError, "the squared norm of no tensors has no device to be on");
     std::vector<odc_span_item> items;
     std::vector<at::Tensor> copies;  // of what is not dense
+    torch::autograd::edge_list inputs;  // a derivative that is asked for is refused, and not silently taken for zero
     items.reserve((size_t)tensors.size());
     const at::Tensor& first = as_tensor(tensors[0], "tensors");
     expect_no_tangent("tensors", first);
@@ -509,6 +512,7 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       expect_no_tangent("tensors", t);
       expect_device("tensors", t, first.device());
       if (float_code("tensors", t) != code) Py_RETURN_NONE;
+      if (t.requires_grad() && at::GradMode::is_enabled()) inputs.push_back(torch::autograd::impl::gradient_edge(t));
       if (t.is_non_overlapping_and_dense()) {
         items.push_back({t.data_ptr(), (uint64_t)t.numel()});
       } else {
@@ -530,6 +534,10 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       check_status(p_squared_norm(items.data(), count, code, workspace.data_ptr(), bytes, static_cast<float*>(result.data_ptr()),
                                   current_stream(first.device())));
     }
+    if (!inputs.empty())
+      torch::autograd::set_history(result, std::shared_ptr<torch::autograd::Error>(
+                                               new torch::autograd::Error("squared_norm: a derivative is not supported", std::move(inputs)),
+                                               torch::autograd::deleteNode));
     return THPVariable_Wrap(std::move(result));
   });
 }

@@ -37,7 +37,7 @@ BLOCK = 32  # elements of a state in 8 bits that share a scale
 def squared_norm(tensors: Sequence[Tensor]) -> Tensor:
     """The sum of the squares of all elements of all tensors, as an fp32 scalar on their device: two launches for up
     to 320 tensors, no round trip to the host. Shards of one model: sum it over the ranks (``all_reduce``) before
-    clipping by it."""
+    clipping by it. It has no derivative: where a tensor requires a gradient, a backward pass through the result raises."""
     if not isinstance(tensors, (list, tuple)):
         tensors = list(tensors)
     total = _host_path.squared_norm(tensors)
