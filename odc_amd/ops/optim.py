@@ -162,7 +162,9 @@ class AdamW(torch.optim.Optimizer):
             grads = [grad for _, _, grads, _ in calls.values() for grad in grads]
             # The norm of this rank's gradients is not that of all ranks'. (Where they are zero they are zero whatever they are clipped by:
             # torch's get_optimizer_state_dict begins the states by such a step.)
-            if any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")) and any(bool(grad.any()) for grad in grads):
+            shards = any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")) or any(
+                _is_flat_shard(p) for owners, _, _, _ in calls.values() for p in owners if hasattr(p, "_unpadded_unsharded_size"))
+            if shards and any(bool(grad.any()) for grad in grads):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
             squared_norm = _host_squared_norm(grads)
         # Every call is checked before the first is made: a step that is refused has written nothing.
@@ -277,6 +279,12 @@ def _first(state: Tensor, elems: int, per: int) -> Tensor:
     elements."""
     local, n = _local(state), -(-elems // per)
     return local if local is state or local.numel() == n else local.view(-1)[:n]
+
+
+def _is_flat_shard(p: Tensor) -> bool:
+    """Whether ``p`` is FSDP1's flat parameter of a model whose other parts are on other ranks. (With ``use_orig_params``
+    the parameters are plain tensors, and nothing says that they are shards.)"""
+    return p.numel() < p._unpadded_unsharded_size.numel()
 
 
 def _local(t: Tensor) -> Tensor:

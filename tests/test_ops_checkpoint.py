@@ -1,4 +1,5 @@
-"""The optimizer's states through torch's distributed checkpoint, on two ranks of the CPU. The kernels are stood in for
+"""The optimizer's states through torch's distributed checkpoint, and shards that need the norm of all ranks, on two
+ranks of the CPU. The kernels are stood in for
 by a step that writes rank and place into every state."""
 
 import itertools
@@ -159,3 +160,24 @@ def test_clipped_shards_are_resumed(tmp_path):
 def test_a_rank_whose_shard_is_empty(tmp_path, bits):
     """One row over two ranks: the second has nothing of it, and states like the first."""
     on_two_ranks(tmp_path, restored, bits, [(8, 32), (1, 32)])
+
+
+def flat_parameters(rank, mesh, path):
+    from torch.distributed.fsdp import FullyShardedDataParallel as FSDP
+
+    from odc_amd.ops import optim
+
+    model = FSDP(torch.nn.Linear(7, 5), device_id=torch.device("cpu"), use_orig_params=False)
+    flat, = model.parameters()
+    assert flat.numel() == 20
+    opt = optim.AdamW([flat], max_norm=1.0)
+    flat.grad = torch.ones_like(flat)
+    with pytest.raises(ValueError, match="shards"):
+        opt.step()
+    opt.step(squared_norm=torch.tensor(40.0))
+    optim.AdamW([flat]).step()  # without clipping there is nothing to know
+
+
+def test_flat_shards_need_the_norm_of_all_ranks(tmp_path):
+    """FSDP1: clipped by its own norm, every rank would take another step."""
+    on_two_ranks(tmp_path, flat_parameters)
