@@ -128,14 +128,14 @@ __device__ __forceinline__ void row_sums(float (&x)[kValues], float* scratch) {
 }
 
 // A row is read once and stays in the registers of its lanes: mean, then the variance about it (not the difference of two large
-// sums), then the output. Weights stay in registers for all rows of a workgroup; the next row is on its way meanwhile: 64 KiB in
-// flight on a CU. 16384 x 4096 bf16 44 us (6.1 TB/s), 4096 x 4096 13.4 (5.0),
+// sums) and what the mean's roundings left, then the output. Weights stay in registers for all rows of a workgroup; the next row is
+// on its way meanwhile: 64 KiB in flight on a CU. 16384 x 4096 bf16 44 us (6.1 TB/s), 4096 x 4096 13.4 (5.0),
 // 16384 x 14336 with a residual 323 (5.8 TB/s), 2048 x 256 fp32 3.0.
 template <class T, class W, int kLanes, int kVectors, RowAccess kAccess, bool kAdd>
 __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads) void norm_forward_kernel(odc_norm_forward c) {
   constexpr int kThreads = kLanes > (int)kForwardThreads ? kLanes : (int)kForwardThreads;
   constexpr int kElems = Vector<T>::kElems;
-  __shared__ float scratch[2][kThreads / 64];
+  __shared__ float scratch[2][2 * kThreads / 64];
   const uint32_t width = (uint32_t)c.width, lane = threadIdx.x % kLanes;
   const float per_element = 1.0f / (float)width;
   Piece<kElems, W, kept(kAccess)> weight[kVectors], bias[kVectors];
@@ -196,21 +196,31 @@ __global__ __launch_bounds__(kLanes > (int)kForwardThreads ? kLanes : (int)kForw
     row += (uint64_t)gridDim.x * kRows;  // the next row is on its way while this one's sums are made
     if constexpr (kAhead) load_row(next);
     row_sums<kLanes>(sum, scratch[0]);
-    const float mean = sum[0] / (float)width;  // (times 1 / width a row of one value would not have it for a mean)
+    const float about = sum[0] / (float)width;  // the mean, but for the sum's roundings
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) x[k].forget();
-    float squares[1] = {};
+    // about it: the squares, and in fp32 what the elements differ by on the average, which is what `about` is off by. (Sums of up to
+    // 32768 values of 8 or 11 bits have hardly a rounding; there the second sum cost 4096 x 4096 bf16 5 % of 12.8 us.)
+    constexpr bool kCorrected = sizeof(T) == 4;
+    float moments[1 + kCorrected] = {};
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
       if (!any_inside<kLanes, kVectors, kElems>(k, width)) continue;
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
-        const float d = (k * kLanes + lane) * kElems + (kAccess != kPlainRows ? 0 : e) < width ? x[k][e] - mean : 0.0f;
-        squares[0] += d * d;
+        const float d = (k * kLanes + lane) * kElems + (kAccess != kPlainRows ? 0 : e) < width ? x[k][e] - about : 0.0f;
+        moments[0] += d * d;
+        if constexpr (kCorrected) moments[1] += d;
       }
     }
-    row_sums<kLanes>(squares, scratch[1]);
-    const float rstd = 1.0f / sqrtf(squares[0] * per_element + c.eps);
+    row_sums<kLanes>(moments, scratch[1]);
+    float mean = about, variance = moments[0] * per_element;
+    if constexpr (kCorrected) {
+      const float off = moments[1] * per_element;
+      mean += off;
+      if (variance < INFINITY) variance = fmaxf(variance - off * off, 0.0f);
+    }
+    const float rstd = 1.0f / sqrtf(variance + c.eps);
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
       if (any_inside<kLanes, kVectors, kElems>(k, width)) {
@@ -423,6 +433,36 @@ __device__ __forceinline__ void store_some(T* row, uint32_t i, uint32_t width, c
   }
 }
 
+// The sum of a vector's values, in pairs (exact for equal values, so that a row of one value has it for a mean; a part of a vector
+// is added one by one for that). What a thread has of a row is added up in 64 bits: in 32, the 2^18 additions of the
+// widest rows would leave a mean that is off by a hundredth.
+template <uint32_t kElems>
+__device__ __forceinline__ double sum_of(const float (&x)[kElems], bool whole = true) {
+  if (!whole) {
+    double sum = x[0];
+#pragma unroll
+    for (uint32_t e = 1; e < kElems; ++e) sum += x[e];
+    return sum;
+  }
+  float pairs[kElems / 2];
+#pragma unroll
+  for (uint32_t e = 0; e < kElems / 2; ++e) pairs[e] = x[2 * e] + x[2 * e + 1];
+#pragma unroll
+  for (uint32_t width = kElems / 4; width; width /= 2)
+#pragma unroll
+    for (uint32_t e = 0; e < width; ++e) pairs[e] += pairs[e + width];
+  return pairs[0];
+}
+
+// The sum over a row's workgroup, in every thread. A row of less than a vector is the first thread's alone.
+__device__ __forceinline__ double wide_sum(double x, bool first_alone, double* scratch) {
+  if (!first_alone) return block_sum<kWideThreads>(x, scratch);
+  __syncthreads();  // the last sum's readers are done
+  if (threadIdx.x == 0) scratch[0] = x;
+  __syncthreads();
+  return scratch[0];
+}
+
 // Weights (or `otherwise` where there are none) beside the elements of a row.
 template <uint32_t kElems, class W>
 __device__ __forceinline__ void load_weights(const W* weights, uint32_t i, uint32_t width, float otherwise, float (&x)[kElems]) {
@@ -444,7 +484,7 @@ __device__ __forceinline__ void load_weights(const W* weights, uint32_t i, uint3
 template <class T, class W>
 __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_norm_forward c) {
   constexpr uint32_t kElems = Vector<T>::kElems, kStep = kWideThreads * kElems;
-  __shared__ float scratch[kWideThreads / 64];
+  __shared__ double scratch[kWideThreads / 64];
   const uint32_t width = (uint32_t)c.width, begin = threadIdx.x * kElems;
   const W* weight = static_cast<const W*>(c.weight);
   const W* bias = static_cast<const W*>(c.bias);
@@ -453,7 +493,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
     const T* r = c.residual ? static_cast<const T*>(c.residual) + row * c.residual_stride : nullptr;
     T* y = static_cast<T*>(c.output) + row * c.width;
     T* total = r ? static_cast<T*>(c.total) + row * c.width : nullptr;
-    float sum = 0;
+    double sum = 0;
     for (uint32_t i = begin; i < width; i += kStep) {
       float v[kElems];
       load_some(x, i, width, v);
@@ -464,22 +504,22 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
         for (uint32_t e = 0; e < kElems; ++e) v[e] = to_float(from_float<T>(v[e] + other[e]));
         store_some(total, i, width, v);
       }
-#pragma unroll
-      for (uint32_t e = 0; e < kElems; ++e) sum += v[e];
+      sum += sum_of(v, i + kElems <= width);
     }
     const T* z = r ? total : x;  // a thread reads what it wrote itself
-    const float mean = block_sum<kWideThreads>(sum, scratch) / (float)width;
-    float squares = 0;
+    const float mean = (float)(wide_sum(sum, width < kElems, scratch) / width);
+    double squares = 0;
     for (uint32_t i = begin; i < width; i += kStep) {
       float v[kElems];
       load_some(z, i, width, v);
 #pragma unroll
       for (uint32_t e = 0; e < kElems; ++e) {
         const float d = i + e < width ? v[e] - mean : 0.0f;
-        squares += d * d;
+        v[e] = d * d;
       }
+      squares += sum_of(v);
     }
-    const float rstd = 1.0f / sqrtf(block_sum<kWideThreads>(squares, scratch) / (float)width + c.eps);
+    const float rstd = 1.0f / sqrtf((float)(wide_sum(squares, width < kElems, scratch) / width) + c.eps);
     for (uint32_t i = begin; i < width; i += kStep) {
       float v[kElems], w[kElems], b[kElems];
       load_some(z, i, width, v);
@@ -499,7 +539,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
 template <class T, class W>
 __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_norm_backward c) {
   constexpr uint32_t kElems = Vector<T>::kElems, kStep = kWideThreads * kElems;
-  __shared__ float scratch[kWideThreads / 64];
+  __shared__ double scratch[kWideThreads / 64];
   const uint32_t width = (uint32_t)c.width, begin = threadIdx.x * kElems;
   const W* weight = static_cast<const W*>(c.weight);
   for (uint64_t row = blockIdx.x; row < c.rows; row += gridDim.x) {
@@ -508,7 +548,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_no
     const T* dt = c.grad_total ? static_cast<const T*>(c.grad_total) + row * c.grad_total_stride : nullptr;
     T* dx = static_cast<T*>(c.grad_input) + row * c.width;
     const float mean = c.mean[row], rstd = c.rstd[row];
-    float sum = 0, dot = 0;
+    double sums = 0, dots = 0;
     for (uint32_t i = begin; i < width; i += kStep) {
       float g[kElems], v[kElems], w[kElems];
       load_some(dy, i, width, g);
@@ -516,13 +556,13 @@ __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_no
       load_weights<kElems>(weight, i, width, 1.0f, w);
 #pragma unroll
       for (uint32_t e = 0; e < kElems; ++e) {
-        const float h = g[e] * w[e];
-        sum += h;
-        dot += h * ((v[e] - mean) * rstd);
+        g[e] *= w[e];
+        v[e] = g[e] * ((v[e] - mean) * rstd);
       }
+      sums += sum_of(g);
+      dots += sum_of(v);
     }
-    sum = block_sum<kWideThreads>(sum, scratch) / (float)width;
-    dot = block_sum<kWideThreads>(dot, scratch) / (float)width;
+    const float sum = (float)(wide_sum(sums, width < kElems, scratch) / width), dot = (float)(wide_sum(dots, width < kElems, scratch) / width);
     for (uint32_t i = begin; i < width; i += kStep) {
       float g[kElems], v[kElems], w[kElems], t[kElems] = {};
       load_some(dy, i, width, g);

@@ -63,10 +63,27 @@ __device__ __forceinline__ float sum_lanes(float x) {
 
 // The sum over the lanes of a wavefront, in every lane.
 __device__ __forceinline__ float wave_sum(float x) { return sum_lanes<64>(x); }
+// In 64 bits the same, a half of the bits at a time.
+__device__ __forceinline__ double of_halves(uint32_t low, uint32_t high) { return __longlong_as_double((long long)((uint64_t)high << 32 | low)); }
+template <int kControl>
+__device__ __forceinline__ double other_lane(double x) {
+  const uint64_t bits = (uint64_t)__double_as_longlong(x);
+  return of_halves(__builtin_amdgcn_update_dpp(0, (uint32_t)bits, kControl, 0xf, 0xf, true),
+                   __builtin_amdgcn_update_dpp(0, (uint32_t)(bits >> 32), kControl, 0xf, 0xf, true));
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+  x += other_lane<0xB1>(x);
+  x += other_lane<0x4E>(x);
+  x += other_lane<0x141>(x);
+  x += other_lane<0x140>(x);
+  uint64_t bits = (uint64_t)__double_as_longlong(x);
+  auto low = __builtin_amdgcn_permlane16_swap((uint32_t)bits, (uint32_t)bits, false, false);
+  auto high = __builtin_amdgcn_permlane16_swap((uint32_t)(bits >> 32), (uint32_t)(bits >> 32), false, false);
+  x = of_halves(low[0], high[0]) + of_halves(low[1], high[1]);
+  bits = (uint64_t)__double_as_longlong(x);
+  low = __builtin_amdgcn_permlane32_swap((uint32_t)bits, (uint32_t)bits, false, false);
+  high = __builtin_amdgcn_permlane32_swap((uint32_t)(bits >> 32), (uint32_t)(bits >> 32), false, false);
+  return of_halves(low[0], high[0]) + of_halves(low[1], high[1]);
 }
 
 // The sum over a workgroup of kThreads, in every thread. `scratch` holds kThreads / 64 values.
