@@ -160,7 +160,7 @@ int odc_adamw(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_num
 /* What odc_adamw would refuse, without a launch: for a step of several calls, all of which are to be made or none. */
 int odc_adamw_check(const odc_adamw_item* items, uint32_t n_items, const odc_adamw_numbers* numbers);
 
-/* values[i] = codes[i] * 2^(scales[i / 32] - 127), in `dtype`. */
+/* values[i] = codes[i] * 2^(scales[i / 32] - 127), in `dtype`; a scale of 255 is not a number. */
 int odc_dequantize_blocks(const void* codes, const void* scales, void* values, uint64_t elems, int32_t dtype,
                           void* stream);
 

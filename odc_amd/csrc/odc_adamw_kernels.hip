@@ -217,7 +217,9 @@ __device__ __forceinline__ float chosen_root(float x, float v, float inverse_sca
   return whole < v * inverse_scale * inverse_scale - below * below ? below + 0.125f * eight : below;
 }
 
-__device__ __forceinline__ float scale_value(uint32_t scale) { return __uint_as_float(scale << 23); }
+// 2^(scale - 127). As an exponent 0 means zero and 255 infinity; with the highest bit of a mantissa they are 2^-127 and not a
+// number, as E8M0 has them.
+__device__ __forceinline__ float scale_value(uint32_t scale) { return __uint_as_float(scale << 23 | ((scale + 1) & 0xFE ? 0 : 0x400000)); }
 
 // Four codes as values, times `factor`.
 __device__ __forceinline__ void values_of(uint32_t codes, float factor, float (&x)[4]) {

@@ -86,8 +86,9 @@ def _norm(squared_norm, max_norm):
 
 
 def dequantize_blocks(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.float32) -> Tensor:
-    """What a state in 8 bits stands for: ``codes * scales``, 32 neighbouring codes to a scale. Exact in bf16 and fp32
-    (4 significant bits times a power of two). Of a sharded parameter's states: what this rank has of them, as long as the
+    """What a state in 8 bits stands for: ``codes * scales``, 32 neighbouring codes to a scale, rounded once into ``dtype``. 4
+    significant bits times a power of two, so it is exact in fp32 up to scales of 2^119, in bf16 with scales of 2^-124 to 2^119: all
+    that the step writes lie there. Of a sharded parameter's states: what this rank has of them, as long as the
     largest shard needs (zeros behind its own)."""
     return _host_path.dequantize_blocks(_local(codes), _local(scales), dtype)
 
