@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -187,10 +188,16 @@ void expect_no_tracing(const char* call) {
 }
 
 // A tangent that the result would not have is one that is taken for zero.
-void expect_no_tangent(const char* what, const at::Tensor& t) {
-  if (t.defined() && t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
-    raise(PyExc_NotImplementedError, "%s: forward-mode derivatives are not supported", what);
-}
+class ForwardMode {
+ public:
+  ForwardMode() : on_(torch::autograd::ForwardADLevel::try_get_by_idx(0) && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {}
+  void expect_no_tangent(const char* what, const at::Tensor& t) const {
+    if (on_ && t.defined() && t._fw_grad(0).defined()) raise(PyExc_NotImplementedError, "%s: forward-mode derivatives are not supported", what);
+  }
+
+ private:
+  bool on_;  // whether any tensor can have one: of hundreds in a list, each is asked only then
+};
 
 void* current_stream(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
@@ -427,10 +434,11 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor input = as_tensor(args[0], "input"), residual = as_optional_tensor(args[1], "residual");
     const at::Tensor weight = as_optional_tensor(args[3], "weight"), bias = as_optional_tensor(args[4], "bias");
     const double eps = as_double(args[5]);
-    expect_no_tangent("input", input);
-    expect_no_tangent("residual", residual);
-    expect_no_tangent("weight", weight);
-    expect_no_tangent("bias", bias);
+    const ForwardMode forward_mode;
+    forward_mode.expect_no_tangent("input", input);
+    forward_mode.expect_no_tangent("residual", residual);
+    forward_mode.expect_no_tangent("weight", weight);
+    forward_mode.expect_no_tangent("bias", bias);
     std::vector<int64_t> shape;
     if (PyLong_Check(args[2])) {
       shape.push_back(as_int(args[2]));
@@ -504,15 +512,17 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     torch::autograd::edge_list inputs;  // a derivative that is asked for is refused, and not silently taken for zero
     items.reserve((size_t)tensors.size());
     const at::Tensor& first = as_tensor(tensors[0], "tensors");
-    expect_no_tangent("tensors", first);
+    const ForwardMode forward_mode;
+    forward_mode.expect_no_tangent("tensors", first);
+    const bool graph = at::GradMode::is_enabled();
     expect_gpu("tensors", first);
     const int32_t code = float_code("tensors", first);
     for (Py_ssize_t k = 0; k < tensors.size(); ++k) {
       const at::Tensor& t = as_tensor(tensors[k], "tensors");
-      expect_no_tangent("tensors", t);
+      forward_mode.expect_no_tangent("tensors", t);
       expect_device("tensors", t, first.device());
       if (float_code("tensors", t) != code) Py_RETURN_NONE;
-      if (t.requires_grad() && at::GradMode::is_enabled()) inputs.push_back(torch::autograd::impl::gradient_edge(t));
+      if (graph && t.requires_grad()) inputs.push_back(torch::autograd::impl::gradient_edge(t));
       if (t.is_non_overlapping_and_dense()) {
         items.push_back({t.data_ptr(), (uint64_t)t.numel()});
       } else {
