@@ -92,10 +92,11 @@ __device__ __forceinline__ float root_of(float v) {
   return small ? r * 0x1p-16f : r;
 }
 
-// The factor of the gradients. A norm that is not a number makes it not a number.
+// The factor of the gradients, one number for all of them: its root and its division are rounded to the nearest. A norm that is
+// not a number makes it not a number.
 __device__ __forceinline__ float factor_of(const AdamwLaunch& launch) {
   if (!launch.squared_norm) return launch.grad_scale;
-  const float c = launch.max_norm * fast_reciprocal(launch.grad_scale * root_of(*launch.squared_norm) + 1e-6f);
+  const float c = launch.max_norm / (launch.grad_scale * sqrtf(*launch.squared_norm) + 1e-6f);
   return launch.grad_scale * (c > 1.0f ? 1.0f : c);
 }
 

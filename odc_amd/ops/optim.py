@@ -16,6 +16,10 @@ a random number, such that its expectation is kept, that of ``m`` and that of ``
 are a function of ``seed``, the tensor's place in the list and the element's in the tensor: the same seed, the same
 bits, another seed for every step. A ``v`` that is not zero is never stored as zero. This step's update is made from
 ``m`` and ``v`` as computed, before they are rounded.
+
+Sums, products and the clipping factor are rounded to the nearest; the root of ``v`` and the reciprocal of the denominator are the
+hardware's, within a unit of the last place each. In 8 bits that can make a code the other neighbour's where its random number is as
+near to the share of the way, as any rounding can.
 """
 
 from __future__ import annotations
