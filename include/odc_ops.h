@@ -114,7 +114,7 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  *
- * (c = 1 where squared_norm is NULL). `copy`, where it is given, receives p in copy_dtype.
+ * (eps is 0 or a normal fp32 number; c = 1 where squared_norm is NULL). `copy`, where it is given, receives p in copy_dtype.
  *
  * state_bits 32: exp_avg and exp_avg_sq are fp32, m and v.
  * state_bits 8: exp_avg and exp_avg_sq hold m and the ROOT of v as OCP e4m3 values; 32 neighbouring

@@ -145,7 +145,7 @@ __device__ __forceinline__ void roots_of(const float (&v)[4], float (&root)[4]) 
   }
 }
 
-// (The denominator is no subnormal number: the root of the smallest v above zero is 3.7e-23.)
+// (The denominator is no subnormal number: the root of the smallest v above zero is 3.7e-23, and eps is none.)
 __device__ __forceinline__ float next_param(const AdamwLaunch& launch, float p, float m, float root) {
   return p * launch.decay - launch.step_size * (m * fast_reciprocal(root * launch.root_scale + launch.eps));
 }

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <limits>
 
 #include "odc_ops.h"
 #include "odc_ops_launch.h"
@@ -260,6 +261,9 @@ int odc_adamw_check(const odc_adamw_item* items, uint32_t n_items, const odc_ada
   if (!(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1)) return fail(ODC_OPS_ERR_INVALID, "the betas lie in [0, 1)");
   if (!(a.eps >= 0) || !(a.lr >= 0) || !(a.weight_decay >= 0) || !std::isfinite(a.eps) || !std::isfinite(a.lr) || !std::isfinite(a.weight_decay))
     return fail(ODC_OPS_ERR_INVALID, "lr, eps and weight_decay are finite and not negative");
+  // (The kernel's reciprocal takes a subnormal number for zero: 0 / eps would not be a number.)
+  if (a.eps > 0 && (float)a.eps < std::numeric_limits<float>::min())
+    return fail(ODC_OPS_ERR_INVALID, "eps is 0 or at least 1.18e-38, the smallest normal fp32 number");
   if (!(a.grad_scale >= 0) || !std::isfinite(a.grad_scale)) return fail(ODC_OPS_ERR_INVALID, "grad_scale is finite and not negative");
   if (a.squared_norm && (!(a.max_norm >= 0) || !aligned(a.squared_norm, 4)))
     return fail(ODC_OPS_ERR_INVALID, "max_norm is not negative, squared_norm aligned to its element");
