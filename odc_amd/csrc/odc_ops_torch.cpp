@@ -211,6 +211,9 @@ void mark_written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Memory that holds a tensor's values: torch puts a sign off (`x.conj().imag`), and the memory then has the other one.
+at::Tensor contiguous(const at::Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+
 // ------------------------------------------------------------------------------------------------
 // layer norm
 // ------------------------------------------------------------------------------------------------
@@ -223,8 +226,8 @@ struct Rows {
   Rows(const at::Tensor& t, int64_t dims, int64_t width) {
     if (!t.defined()) return;
     tensor = t;
-    if (row_stride(t, dims, width, &stride)) return;
-    tensor = t.contiguous();
+    if (!t.is_neg() && row_stride(t, dims, width, &stride)) return;
+    tensor = contiguous(t);
     stride = (uint64_t)width;
   }
 
@@ -262,8 +265,6 @@ struct NormOutputs {
 };
 
 void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-at::Tensor contiguous(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 NormOutputs norm_forward(const at::Tensor& input, const at::Tensor& residual, const at::Tensor& weight, const at::Tensor& bias,
                          const NormShape& shape, double eps, bool keep_statistics) {
@@ -552,6 +553,11 @@ PyObject* squared_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// A tensor that is written is its memory (contiguous()).
+void expect_no_sign_put_off(const char* name, const at::Tensor& t, Py_ssize_t k) {
+  if (t.is_neg()) raise(PyExc_ValueError, "%s: tensor %zd is a view whose sign was put off: it cannot be written", name, k);
+}
+
 bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   if (a.dim() == 1 && b.dim() == 1) return a.numel() == b.numel() && a.is_contiguous() && b.is_contiguous();
   return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
@@ -580,7 +586,16 @@ class Beside {
     if (!given_) return nullptr;
     const at::Tensor& t = at(k, param.device());
     if (!same_layout(t, param)) raise(PyExc_ValueError, "%s: tensor %zd is not laid out as its parameter is", name_, k);
+    expect_no_sign_put_off(name_, t, k);
     return t.data_ptr();
+  }
+
+  // the same, of what is only read
+  const void* read_like(Py_ssize_t k, const at::Tensor& param) {
+    if (!THPVariable_Check(items_[k]) || !THPVariable_Unpack(items_[k]).is_neg()) return like(k, param);
+    resolved_.push_back(at(k, param.device()).resolve_neg());
+    if (!same_layout(resolved_.back(), param)) raise(PyExc_ValueError, "%s: tensor %zd is not laid out as its parameter is", name_, k);
+    return resolved_.back().data_ptr();
   }
 
   // `numel` values in the order of the memory
@@ -608,6 +623,7 @@ class Beside {
   const char* name_;
   bool given_;
   Sequence items_;
+  std::vector<at::Tensor> resolved_;
   at::ScalarType dtype_ = at::kByte;
 };
 
@@ -661,11 +677,12 @@ class AdamwCall {
       expect_device("params", p, first.device());
       if (p.scalar_type() != first.scalar_type()) raise(PyExc_TypeError, "params: tensors of one call have one dtype");
       if (!p.is_non_overlapping_and_dense()) raise(PyExc_ValueError, "params: tensor %zd is not dense", k);
+      expect_no_sign_put_off("params", p, k);
       odc_adamw_item item = {};
       const int64_t numel = p.numel(), blocks = (numel + kBlock - 1) / kBlock;
       item.elems = (uint64_t)numel;
       item.param = p.data_ptr();
-      item.grad = grads_.like(k, p);
+      item.grad = grads_.read_like(k, p);
       item.exp_avg = eight ? m_.flat(k, p.device(), numel) : m_.like(k, p);
       item.exp_avg_sq = eight ? v_.flat(k, p.device(), numel) : v_.like(k, p);
       item.exp_avg_scale = m_scale_.flat(k, p.device(), blocks);
@@ -688,6 +705,7 @@ class AdamwCall {
     for (const Beside* states : {&m_, &v_}) states->expect(eight ? at::kFloat8_e4m3fn : at::kFloat);
     for (const Beside* scales : {&m_scale_, &v_scale_}) scales->expect(at::kFloat8_e8m0fnu);
     if (squared_norm_.defined()) {
+      squared_norm_ = squared_norm_.resolve_neg();
       expect_device("squared_norm", squared_norm_, first.device());
       if (squared_norm_.numel() != 1 || squared_norm_.scalar_type() != at::kFloat) raise(PyExc_TypeError, "squared_norm: expected one fp32 value");
       numbers_.squared_norm = static_cast<const float*>(squared_norm_.data_ptr());
