@@ -454,6 +454,15 @@ __device__ __forceinline__ double sum_of(const float (&x)[kElems], bool whole = 
   return pairs[0];
 }
 
+// Calls body with the first elements of a thread's vectors in a row: the whole ones in a loop, whose condition is the one that
+// load_some and store_some ask for, and the one that the row's end cuts behind it.
+template <uint32_t kElems, class Body>
+__device__ __forceinline__ void over_row(uint32_t begin, uint32_t width, Body body) {
+  uint32_t i = begin;
+  for (; i + kElems <= width; i += kWideThreads * kElems) body(i);
+  if (i < width) body(i);
+}
+
 // The sum over a row's workgroup, in every thread. A row of less than a vector is the first thread's alone.
 __device__ __forceinline__ double wide_sum(double x, bool first_alone, double* scratch) {
   if (!first_alone) return block_sum<kWideThreads>(x, scratch);
@@ -483,7 +492,7 @@ __device__ __forceinline__ void load_weights(const W* weights, uint32_t i, uint3
 // columns, 360 + 134; in bf16 138 + 75.
 template <class T, class W>
 __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_norm_forward c) {
-  constexpr uint32_t kElems = Vector<T>::kElems, kStep = kWideThreads * kElems;
+  constexpr uint32_t kElems = Vector<T>::kElems;
   __shared__ double scratch[kWideThreads / 64];
   const uint32_t width = (uint32_t)c.width, begin = threadIdx.x * kElems;
   const W* weight = static_cast<const W*>(c.weight);
@@ -494,7 +503,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
     T* y = static_cast<T*>(c.output) + row * c.width;
     T* total = r ? static_cast<T*>(c.total) + row * c.width : nullptr;
     double sum = 0;
-    for (uint32_t i = begin; i < width; i += kStep) {
+    over_row<kElems>(begin, width, [&](uint32_t i) {
       float v[kElems];
       load_some(x, i, width, v);
       if (r) {
@@ -505,11 +514,11 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
         store_some(total, i, width, v);
       }
       sum += sum_of(v, i + kElems <= width);
-    }
+    });
     const T* z = r ? total : x;  // a thread reads what it wrote itself
     const float mean = (float)(wide_sum(sum, width < kElems, scratch) / width);
     double squares = 0;
-    for (uint32_t i = begin; i < width; i += kStep) {
+    over_row<kElems>(begin, width, [&](uint32_t i) {
       float v[kElems];
       load_some(z, i, width, v);
 #pragma unroll
@@ -518,9 +527,9 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
         v[e] = d * d;
       }
       squares += sum_of(v);
-    }
+    });
     const float rstd = 1.0f / sqrtf((float)(wide_sum(squares, width < kElems, scratch) / width) + c.eps);
-    for (uint32_t i = begin; i < width; i += kStep) {
+    over_row<kElems>(begin, width, [&](uint32_t i) {
       float v[kElems], w[kElems], b[kElems];
       load_some(z, i, width, v);
       load_weights<kElems>(weight, i, width, 1.0f, w);
@@ -528,7 +537,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
 #pragma unroll
       for (uint32_t e = 0; e < kElems; ++e) v[e] = (v[e] - mean) * rstd * w[e] + b[e];
       store_some(y, i, width, v);
-    }
+    });
     if (threadIdx.x == 0) {
       if (c.mean) c.mean[row] = mean;
       if (c.rstd) c.rstd[row] = rstd;
@@ -538,7 +547,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_nor
 
 template <class T, class W>
 __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_norm_backward c) {
-  constexpr uint32_t kElems = Vector<T>::kElems, kStep = kWideThreads * kElems;
+  constexpr uint32_t kElems = Vector<T>::kElems;
   __shared__ double scratch[kWideThreads / 64];
   const uint32_t width = (uint32_t)c.width, begin = threadIdx.x * kElems;
   const W* weight = static_cast<const W*>(c.weight);
@@ -549,7 +558,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_no
     T* dx = static_cast<T*>(c.grad_input) + row * c.width;
     const float mean = c.mean[row], rstd = c.rstd[row];
     double sums = 0, dots = 0;
-    for (uint32_t i = begin; i < width; i += kStep) {
+    over_row<kElems>(begin, width, [&](uint32_t i) {
       float g[kElems], v[kElems], w[kElems];
       load_some(dy, i, width, g);
       load_some(x, i, width, v);
@@ -561,9 +570,9 @@ __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_no
       }
       sums += sum_of(g);
       dots += sum_of(v);
-    }
+    });
     const float sum = (float)(wide_sum(sums, width < kElems, scratch) / width), dot = (float)(wide_sum(dots, width < kElems, scratch) / width);
-    for (uint32_t i = begin; i < width; i += kStep) {
+    over_row<kElems>(begin, width, [&](uint32_t i) {
       float g[kElems], v[kElems], w[kElems], t[kElems] = {};
       load_some(dy, i, width, g);
       load_some(x, i, width, v);
@@ -572,7 +581,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_backward_rows_kernel(odc_no
 #pragma unroll
       for (uint32_t e = 0; e < kElems; ++e) v[e] = rstd * (g[e] * w[e] - sum - (v[e] - mean) * rstd * dot) + t[e];
       store_some(dx, i, width, v);
-    }
+    });
   }
 }
 
