@@ -116,7 +116,15 @@ NormBackwardPlan backward_plan(uint64_t rows, uint64_t width, int32_t dtype) {
     plan.groups = rows && rounds <= kRoundsAlone ? 1 : (uint32_t)std::min(rounds, kCus);
     plan.rows_per_group = 0;
   } else {
-    plan.rows_per_group = std::max<uint64_t>(1, ceil_div(rows, kCus));
+    // The pass over columns: a row at least for each wavefront of a group, and no more groups, whose sums go to memory and back,
+    // than 1024 workgroups need, or 32 rows to a wavefront in long columns. us of the backward pass in bf16 by this rule /
+    // with up to 256 groups / with 1024 workgroups whatever the rows: 1000 x 20000 49 / 61 / 49, 4096 x 20000 196 / 210 / 200,
+    // 100000 x 20000 4417 / 4420 / 4977, 256 x 1000000 1042 / 1066 / 1027. (A group for every row, of which a wavefront in
+    // four has any, makes a workspace of four times the input: 300 x 20000 39 instead of 25.)
+    constexpr uint64_t kWaves = kWideThreads / 64, kWorkgroups = 1024, kRows = 32;
+    const uint64_t tiles = ceil_div(width, 64 * (16 / bytes_of(dtype)));
+    const uint64_t groups = std::min({ceil_div(rows, kWaves), std::max(ceil_div(kWorkgroups, tiles), ceil_div(rows, kWaves * kRows)), kCus});
+    plan.rows_per_group = rows ? ceil_div(rows, groups) : 1;
     plan.groups = (uint32_t)ceil_div(rows, plan.rows_per_group);
   }
   return plan;
