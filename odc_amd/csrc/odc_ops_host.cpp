@@ -137,7 +137,7 @@ uint32_t fill_table(Launch& launch, const Item* items, uint32_t n_items, uint32_
   launch.n_items = launch.n_tiles = 0;
   while (at < n_items && launch.n_items < most_items) {
     const uint64_t tiles = ceil_div(items[at].elems, tile);
-    if (tiles > most_workgroups(threads) - launch.n_tiles) break;  // (one tensor alone always fits: check_list)
+    if (tiles > most_workgroups(threads) - launch.n_tiles) break;  // (one tensor alone always fits: check_elems)
     launch.first_tile[launch.n_items] = launch.n_tiles;
     launch.set(launch.n_items++, items[at++]);
     launch.n_tiles += (uint32_t)tiles;
@@ -235,8 +235,9 @@ int odc_squared_norm(const odc_span_item* items, uint32_t n_items, int32_t dtype
   if (!is_float_type(dtype)) return fail(ODC_OPS_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
   for (uint32_t i = 0; i < n_items; ++i) {
     ODC_OPS_TRY(check_elems(items[i].elems, i, kNormTile, kNormThreads));
-    if (items[i].elems && (!items[i].data || !aligned(items[i].data, bytes_of(dtype)) || (uint64_t)(uintptr_t)items[i].data >> 48))
-      return fail(ODC_OPS_ERR_INVALID, "item %u: data is NULL or not aligned to its element", i);
+    if (!items[i].elems) continue;
+    if (!items[i].data || !aligned(items[i].data, bytes_of(dtype))) return fail(ODC_OPS_ERR_INVALID, "item %u: data is NULL or not aligned to its element", i);
+    if ((uint64_t)(uintptr_t)items[i].data >> 48) return fail(ODC_OPS_ERR_INVALID, "item %u: an address above 48 bits is no address of a GPU's", i);
   }
   const uint64_t need = n_items ? odc_squared_norm_workspace(items, n_items, dtype) : 0;
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))

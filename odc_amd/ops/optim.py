@@ -167,8 +167,9 @@ class AdamW(torch.optim.Optimizer):
             grads = [grad for _, _, grads, _ in calls.values() for grad in grads]
             # The norm of this rank's gradients is not that of all ranks'. (Where they are zero they are zero whatever they are clipped by:
             # torch's get_optimizer_state_dict begins the states by such a step.)
-            shards = any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh")) or any(
-                _is_flat_shard(p) for owners, _, _, _ in calls.values() for p in owners if hasattr(p, "_unpadded_unsharded_size"))
+            shards = torch.distributed.is_available() and torch.distributed.is_initialized() and (
+                any(p.device_mesh.size() > 1 for p in sharded if hasattr(p, "device_mesh"))
+                or any(_is_flat_shard(p) for owners, _, _, _ in calls.values() for p in owners if hasattr(p, "_unpadded_unsharded_size")))
             if shards and any(bool(grad.any()) for grad in grads):
                 raise ValueError("the parameters are shards: give step() the squared_norm of their gradients, summed over the ranks")
             squared_norm = _host_squared_norm(grads)
