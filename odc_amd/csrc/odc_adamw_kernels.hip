@@ -1,9 +1,10 @@
 // odc_adamw_kernels.hip — the squared norm and the AdamW step of many tensors for gfx950.
 //
 // The formulas are in include/odc_ops.h. All of it is one pass over memory: 28 bytes for an element of an fp32 step, 16.1 with states
-// in 8 bits, 10.1 with bf16 parameters and gradients beside those. HBM bounds all but the last, which its 86 instructions do.
-// Measured: fp32 4.33 ms over 1.0 G elements (6.5 TB/s); 8 bits 67 us over 27.3 M (6.6 TB/s); bf16 with 8 bits 31 us over 11.2 M
-// (3.6 TB/s); the squared norm 287 us over 1.0 G bf16 elements (7.0 TB/s), 7.4 us over 300 small tensors.
+// in 8 bits, 10.1 with bf16 parameters and gradients beside those. HBM bounds all but the last, which its 88 instructions do.
+// Measured: fp32 4.33 to 4.50 ms over 1.0 G elements (6.2 to 6.5 TB/s), with bf16 parameters and gradients 333 us over 100 M (6.6 TB/s
+// at 22 bytes); 8 bits 67 to 70 us over 27.3 M (6.3 to 6.6 TB/s); bf16 with 8 bits 31 us over 11.2 M (3.6 TB/s); the squared norm
+// 287 us over 1.0 G bf16 elements (7.0 TB/s), 7.2 us over 300 small tensors.
 #include <type_traits>
 
 #include "odc_ops_device.h"

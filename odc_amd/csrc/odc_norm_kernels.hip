@@ -488,8 +488,8 @@ __device__ __forceinline__ void load_weights(const W* weights, uint32_t i, uint3
 }
 
 // One workgroup per row, three passes over it (the second and third find it in the caches): the mean, the
-// variance about that mean, the output. 4096 x 20000 fp32 with a residual 380 us (3.4 TB/s); backward, the rows and then the
-// columns, 360 + 134; in bf16 138 + 75.
+// variance about that mean, the output. 4096 x 20000 fp32 with a residual 354 us (3.7 TB/s); backward, the rows and then the
+// columns, 266 + 133; in bf16 123 + 69. (Rows of less than a vector: 1000000 x 4 bf16 2.8 ms, one lane of a workgroup has work.)
 template <class T, class W>
 __global__ __launch_bounds__(kWideThreads) void norm_forward_wide_kernel(odc_norm_forward c) {
   constexpr uint32_t kElems = Vector<T>::kElems;

@@ -100,8 +100,8 @@ struct AdamwShape {
 // In fp32 four streams are read and three written, and what bounds them is how HBM mixes these: it likes few bytes in
 // flight. us over 1.0 G elements / over 27 M with clipping and a copy, of which a part stays in the last-level cache: one
 // wavefront of 256 elements at a time, 3 to a SIMD 4411 / 142 (6.4 TB/s), 4 4500 / 140, 8 4619 / 143; 128 threads 4655 / 139;
-// 256 threads 4897 / 139; two vectors to a lane 5143 / 142. States in 8 bits have arithmetic to hide, about 70 instructions for
-// an element: 256 threads x 2 144, x 1 148, 64 x 2 147 us over 27 M with clipping.
+// 256 threads 4897 / 139; two vectors to a lane 5143 / 142. States in 8 bits have arithmetic to hide, 78 instructions for
+// an element: 256 threads x 2 130, x 1 132, 64 x 2 132 us over 27 M with clipping and values read out.
 constexpr AdamwShape adamw_shape(bool eight) { return eight ? AdamwShape{256, 2, 8} : AdamwShape{64, 1, 3}; }
 constexpr uint32_t kAdamwWords = 400;
 struct AdamwLaunch {
