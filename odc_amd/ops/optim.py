@@ -61,12 +61,12 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     copies; 57 and 50 with states in 8 bits).
 
     ``params`` are fp32 or bf16, ``grads`` fp32, bf16 or fp16, the states fp32; every list has one dtype, and the
-    tensors of a place have one shape and layout, dense, at any alignment. ``step`` counts from 1. ``squared_norm``
-    (a scalar on the device, see the function) and ``max_norm`` come together and clip the gradients;
-    ``grad_scale`` multiplies them first (1 / W for sums over W ranks). A norm that is not finite is not looked at by the
-    host: NaN makes every parameter NaN, as the formula says. ``copies`` (bf16 or fp16, of fp32 parameters)
-    receive the new parameters. Parameters in bf16 are rounded to the nearest value, which loses updates of less than
-    half a unit in their last place, or, where ``seed`` is given, by its random numbers."""
+    tensors of a place have one shape and layout, dense, at any alignment; what is written overlaps nothing else of the
+    call. ``step`` counts from 1. ``squared_norm`` (a scalar on the device, see the function) and ``max_norm`` come
+    together and clip the gradients; ``grad_scale`` multiplies them first (1 / W for sums over W ranks). A norm that is not
+    finite is not looked at by the host: NaN makes every parameter NaN, as the formula says. ``copies`` (bf16 or fp16, of
+    fp32 parameters) receive the new parameters. Parameters in bf16 are rounded to the nearest value, which loses updates
+    of less than half a unit in their last place, or, where ``seed`` is given, by its random numbers."""
     _host_path.adamw(params, grads, exp_avgs, None, exp_avg_sqs, None, copies, _norm(squared_norm, max_norm), step, lr, *betas, eps,
                      weight_decay, grad_scale, 0.0 if max_norm is None else max_norm, seed)
 
