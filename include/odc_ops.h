@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define ODC_OPS_ABI_VERSION 1
+#define ODC_OPS_ABI_VERSION 2
 
 typedef enum odc_ops_status {
   ODC_OPS_OK = 0,

@@ -77,7 +77,7 @@ OPS_EXPORTED_SYMBOLS = (
 )
 
 ABI_VERSION = 3
-OPS_ABI_VERSION = 1
+OPS_ABI_VERSION = 2
 MAX_ITEMS_PER_LAUNCH = 112
 
 ODC_OK = 0
